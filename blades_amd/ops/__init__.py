@@ -240,6 +240,16 @@ def centered_clip_iter(U: Tensor, v: Tensor, tau: float) -> Tensor:
     return _ref.centered_clip_iter(U, v, tau)
 
 
+# ------------------------------------------------- token-model operators
+
+from .token import (  # noqa: E402  (uses the dispatch above)
+    gelu_act8,
+    layer_norm,
+    linear_act8,
+    linear_cross_entropy,
+)
+
+
 __all__ = [
     "col_mean", "col_median", "trimmed_mean", "col_var",
     "weighted_col_sum", "masked_col_mean", "masked_col_mean_std",
@@ -248,4 +258,5 @@ __all__ = [
     "krum_scores", "col_trimmed_sum",
     "clip_to_norm", "centered_clip_iter", "row_clip_to_norm_",
     "philox_normal", "flat_sgd_step_", "sanitize_", "hip_available",
+    "layer_norm", "linear_cross_entropy", "gelu_act8", "linear_act8",
 ]

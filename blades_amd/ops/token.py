@@ -1,0 +1,511 @@
+"""Training operators of token models (text and image transformers).
+
+* :func:`layer_norm` — forward and backward, the parameters' gradients summed
+  per client;
+* :func:`linear_cross_entropy` — cross entropy of a linear head over a large
+  vocabulary, without keeping its logits;
+* :func:`gelu_act8`, :func:`linear_act8` — GELU and linear layers that keep
+  their input in 8 bits for the backward pass.
+
+float32 and bfloat16.  GPU tensors run the HIP kernels of ``csrc/`` (and
+refuse to run without them), CPU tensors the plain forms of
+:mod:`torch_ref`.  Every operator runs under ``torch.func.grad`` and
+``torch.func.vmap`` in either nesting: a vmapped call is ONE launch over all
+clients ("groups" below), with shared or per-client parameters, and
+``vmap(grad(...))`` gets the parameters' gradients per client from the
+kernels.  A vmap inside a vmap whose parameters or gradients are per client at
+both levels is refused.  The operators' gradients are not differentiable
+again.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch._C import _functorch
+from torch.autograd import Function
+
+from . import torch_ref as _ref
+
+Tensor = torch.Tensor
+
+_DTYPES = (torch.float32, torch.bfloat16)
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _kernels(t: Tensor):
+    from blades_amd import ops
+
+    return ops._route(t) or _ref
+
+
+# ------------------------------------------------------------------ checks
+
+def _check_input(name: str, x: Tensor, min_dim: int = 1) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {x.dtype}")
+    if x.dim() < min_dim:
+        raise ValueError(f"{name} needs at least {min_dim} dimension(s), got "
+                         f"shape {tuple(x.shape)}")
+    if x.shape[-1] == 0:
+        raise ValueError(f"{name} has an empty last axis")
+
+
+def _check_param(name: str, p: Optional[Tensor], x: Tensor, shape) -> None:
+    if p is None:
+        return
+    if not isinstance(p, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(p).__name__}")
+    if p.dtype != x.dtype:
+        raise TypeError(f"{name} must have x's type {x.dtype}, got {p.dtype}")
+    if p.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {p.device}")
+    if tuple(p.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got "
+                         f"{tuple(p.shape)}")
+
+
+# ------------------------------------------------------------- vmap helpers
+
+def _batched(t, dim, size: int):
+    """``t`` with its client axis first; a tensor without one is repeated."""
+    if t is None:
+        return None
+    return t.movedim(dim, 0) if dim is not None else t.expand(size, *t.shape)
+
+
+def _param_batched(t, dim):
+    """Client axis first, or left shared."""
+    return t if t is None or dim is None else t.movedim(dim, 0)
+
+
+def _refuse_nested(groups: int, op: str) -> None:
+    if groups:
+        raise NotImplementedError(
+            f"{op}: a vmap over clients inside another vmap is not supported")
+
+
+def _groups3(t: Tensor, groups: int) -> Tensor:
+    """[groups or 1, rows, last] contiguous."""
+    lead = groups if groups else 1
+    rows = t[0].numel() // t.shape[-1] if groups and t.shape[0] else (
+        t.numel() // t.shape[-1])
+    return t.reshape(lead, rows, t.shape[-1]).contiguous()
+
+
+class _NoSecond(Function):
+    """Base of the gradient functions."""
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(
+            "the gradients of blades_amd.ops token operators are not "
+            "differentiable again")
+
+
+# -------------------------------------------------------------- layer norm
+
+class _NormGrad(_NoSecond):
+    @staticmethod
+    def forward(dy, x, w, mean, rstd, groups, params):
+        g = max(groups, 1)
+        dx, dw, db = _kernels(x).norm_backward(
+            _groups3(dy, groups), _groups3(x, groups),
+            mean.reshape(g, -1).contiguous(),
+            rstd.reshape(g, -1).contiguous(),
+            None if w is None else w.contiguous(), params)
+        if not groups and params:
+            dw, db = dw[0], db[0]
+        return dx.view(x.shape), dw, db
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, dy, x, w, mean, rstd, groups, params):
+        _refuse_nested(groups, "layer_norm")
+        n = info.batch_size
+        out = _NormGrad.apply(
+            _batched(dy, in_dims[0], n), _batched(x, in_dims[1], n),
+            _param_batched(w, in_dims[2]), _batched(mean, in_dims[3], n),
+            _batched(rstd, in_dims[4], n), n, params)
+        per = 0 if params else None
+        return out, (0, per, per)
+
+
+class _Norm(Function):
+    # groups: 0, or the number of clients on x's first axis with parameters of
+    # their own in w and b
+
+    @staticmethod
+    def forward(x, w, b, eps, groups):
+        y, mean, rstd = _kernels(x).norm_forward(
+            _groups3(x, groups), None if w is None else w.contiguous(),
+            None if b is None else b.contiguous(), eps)
+        lead = x.shape[:-1]
+        return y.view(x.shape), mean.view(lead), rstd.view(lead)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, b, _, groups = inputs
+        _, mean, rstd = output
+        ctx.mark_non_differentiable(mean, rstd)
+        ctx.save_for_backward(x, w, mean, rstd)
+        ctx.groups = groups
+        ctx.has_b = b is not None
+
+    @staticmethod
+    def backward(ctx, dy, _mean, _rstd):
+        x, w, mean, rstd = ctx.saved_tensors
+        need_w = w is not None and ctx.needs_input_grad[1]
+        need_b = ctx.has_b and ctx.needs_input_grad[2]
+        dx, dw, db = _NormGrad.apply(dy, x, w, mean, rstd, ctx.groups,
+                                     need_w or need_b)
+        return (dx, dw if need_w else None, db if need_b else None, None,
+                None)
+
+    @staticmethod
+    def vmap(info, in_dims, x, w, b, eps, groups):
+        _refuse_nested(groups, "layer_norm")
+        n = info.batch_size
+        x = _batched(x, in_dims[0], n)
+        if in_dims[1] is not None or in_dims[2] is not None:
+            w, b, groups = (_batched(w, in_dims[1], n),
+                            _batched(b, in_dims[2], n), n)
+        return _Norm.apply(x, w, b, eps, groups), (0, 0, 0)
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None,
+               bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """Normalise ``x`` [..., dim] over its last axis, then scale and shift.
+
+    ``weight``, ``bias``: [dim] in x's type, or None.  Statistics and the
+    sums of the gradients are 32-bit; each output is rounded once.
+    """
+    _check_input("x", x)
+    _check_param("weight", weight, x, x.shape[-1:])
+    _check_param("bias", bias, x, x.shape[-1:])
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    return _Norm.apply(x, weight, bias, float(eps), 0)[0]
+
+
+# -------------------------------------------------------- head cross entropy
+
+class _HeadLossGrad(_NoSecond):
+    @staticmethod
+    def forward(grad, x, w, b, target, lse, count, ignore, reduction, groups,
+                wants):
+        g = max(groups, 1)
+        dx, dw, db = _kernels(x).loss_backward(
+            grad.float().reshape(g, -1).contiguous(), _groups3(x, groups),
+            w.contiguous(), target.reshape(g, -1).contiguous(),
+            None if b is None else b.contiguous(),
+            lse.reshape(g, -1).contiguous(), count.reshape(g).contiguous(),
+            ignore, reduction, *wants)
+        if not groups:
+            dw = dw[0] if wants[1] else dw
+            db = db[0] if wants[2] else db
+        return (dx.view(x.shape) if wants[0] else dx), dw, db
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, grad, x, w, b, target, lse, count, ignore,
+             reduction, groups, wants):
+        _refuse_nested(groups, "linear_cross_entropy")
+        n = info.batch_size
+        out = _HeadLossGrad.apply(
+            _batched(grad, in_dims[0], n), _batched(x, in_dims[1], n),
+            _param_batched(w, in_dims[2]), _param_batched(b, in_dims[3]),
+            _batched(target, in_dims[4], n), _batched(lse, in_dims[5], n),
+            _batched(count, in_dims[6], n), ignore, reduction, n, wants)
+        return out, tuple(0 if want else None for want in wants)
+
+
+class _HeadLoss(Function):
+    # groups: 0, or the number of clients on the first axis of x and target;
+    # w and b are then shared or per client
+
+    @staticmethod
+    def forward(x, w, b, target, ignore, reduction, groups):
+        g = max(groups, 1)
+        loss, lse, count = _kernels(x).loss_forward(
+            _groups3(x, groups), w.contiguous(),
+            target.reshape(g, -1).contiguous(),
+            None if b is None else b.contiguous(), ignore, reduction)
+        if reduction == 0:
+            loss = loss.view(target.shape)
+        elif not groups:
+            loss = loss[0]
+        return (loss, lse.view(target.shape),
+                count if groups else count[0])
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, b, target, ignore, reduction, groups = inputs
+        _, lse, count = output
+        ctx.mark_non_differentiable(lse, count)
+        ctx.save_for_backward(x, w, b, target, lse, count)
+        ctx.settings = (ignore, reduction, groups)
+
+    @staticmethod
+    def backward(ctx, grad, _lse, _count):
+        x, w, b, target, lse, count = ctx.saved_tensors
+        ignore, reduction, groups = ctx.settings
+        wants = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                 b is not None and ctx.needs_input_grad[2])
+        if groups and w.dim() == 2:
+            # shared parameters: one sum over all clients' rows, each row
+            # with its client's share of the upstream gradient
+            if reduction == 2:
+                grad = grad / count
+            if reduction != 0:
+                ones = (1,) * (target.dim() - 1)
+                grad = grad.view(-1, *ones).expand(target.shape)
+            reduction, groups, count = 0, 0, count[:1]
+        dx, dw, db = _HeadLossGrad.apply(grad, x, w, b, target, lse, count,
+                                         ignore, reduction, groups, wants)
+        return (dx if wants[0] else None, dw if wants[1] else None,
+                db if wants[2] else None, None, None, None, None)
+
+    @staticmethod
+    def vmap(info, in_dims, x, w, b, target, ignore, reduction, groups):
+        _refuse_nested(groups, "linear_cross_entropy")
+        n = info.batch_size
+        x = _batched(x, in_dims[0], n)
+        target = _batched(target, in_dims[3], n)
+        if in_dims[1] is not None or in_dims[2] is not None:
+            w, b = _batched(w, in_dims[1], n), _batched(b, in_dims[2], n)
+        return (_HeadLoss.apply(x, w, b, target, ignore, reduction, n),
+                (0, 0, 0))
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
+                         bias: Optional[Tensor] = None,
+                         ignore_index: int = -100,
+                         reduction: str = "mean") -> Tensor:
+    """Cross entropy of the logits ``x @ weight.T + bias`` with ``target``,
+    in float32, computed in tiles: the [rows, vocab] logits are never stored.
+    The backward pass computes them again, a piece of the vocabulary at a
+    time (at most 256 MiB of their gradient exists at once, or 512 words).
+
+    ``x``: [..., dim]; ``weight``: [vocab, dim]; ``bias``: [vocab] or None;
+    ``target``: int64, x's leading shape.  Rows whose target is
+    ``ignore_index`` have loss 0 and no gradient.  ``reduction``: ``"none"``
+    (target's shape), ``"sum"``, or ``"mean"`` over the rows that count (NaN
+    where none does, as torch has it; their gradient is zero).
+
+    A target outside the vocabulary cannot raise without stopping the GPU's
+    stream: its row's loss, and every gradient it enters, is NaN.  ``bias``
+    may hold -inf for words that are switched off.
+    """
+    _check_input("x", x)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be a [vocab, dim] tensor")
+    if weight.shape[0] == 0:
+        raise ValueError("weight has no rows")
+    _check_param("weight", weight, x, (weight.shape[0], x.shape[-1]))
+    _check_param("bias", bias, x, weight.shape[:1])
+    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64:
+        raise TypeError("target must be an int64 tensor")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target must have shape {tuple(x.shape[:-1])}, got "
+                         f"{tuple(target.shape)}")
+    if target.device != x.device:
+        raise ValueError(f"target must be on {x.device}, got {target.device}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}, got "
+                         f"{reduction!r}")
+    return _HeadLoss.apply(x, weight, bias, target, int(ignore_index),
+                           _REDUCTIONS.index(reduction), 0)[0]
+
+
+# ------------------------------------------------- 8-bit activation storage
+
+class _GeluGrad(_NoSecond):
+    @staticmethod
+    def forward(dy, q, e):
+        return _kernels(dy).gelu_backward(dy.contiguous(), q.contiguous(),
+                                          e.contiguous())
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, dy, q, e):
+        n = info.batch_size
+        return _GeluGrad.apply(*(_batched(t, d, n) for t, d in
+                                 zip((dy, q, e), in_dims))), 0
+
+
+class _Gelu8(Function):
+    @staticmethod
+    def forward(x, keep):
+        return tuple(_kernels(x).gelu_forward(x.contiguous(), keep))
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, q, e = output
+        ctx.mark_non_differentiable(q, e)
+        ctx.save_for_backward(q, e)
+
+    @staticmethod
+    def backward(ctx, dy, _q, _e):
+        q, e = ctx.saved_tensors
+        return _GeluGrad.apply(dy, q, e), None
+
+    @staticmethod
+    def vmap(info, in_dims, x, keep):
+        per = 0 if keep else None
+        return (_Gelu8.apply(_batched(x, in_dims[0], info.batch_size), keep),
+                (0, per, per))
+
+
+def gelu_act8(x: Tensor) -> Tensor:
+    """GELU, ``x * Phi(x)``, that keeps ``x`` in 8 bits for its gradient.
+
+    Along the last axis every 128 values share the least power of two
+    ``2**e`` (e >= -126) with ``max|x| <= 127 * 2**e`` and are held as int8:
+    1.008 bytes a value.  The gradient is the formula's at the values held,
+    which differ from ``x`` by at most ``2**(e-1)``; a block of 128 that
+    holds an infinity or NaN has gradient NaN.  The output comes from ``x``
+    itself.
+    """
+    _check_input("x", x)
+    return _Gelu8.apply(x, _tracks(x))[0]
+
+
+def _tracks(t: Tensor) -> bool:
+    """Whether a gradient of ``t`` can be asked for, at any level of the
+    torch.func transforms around the call."""
+    if not torch.is_grad_enabled():
+        return False
+    while not t.requires_grad:
+        if not _functorch.is_functorch_wrapped_tensor(t):
+            return False
+        t = _functorch.get_unwrapped(t)
+    return True
+
+
+def _product(x: Tensor, w: Tensor, groups: int, transpose: bool, b=None):
+    """x @ w.T + b (or x @ w) with shared or per-client w."""
+    k = _kernels(x)
+    x3 = _groups3(x, groups)
+    n = w.shape[-2] if transpose else w.shape[-1]
+    if (x.is_cuda and k is not _ref and w.dim() == 2
+            and x.dtype == torch.bfloat16):
+        # one plain bf16 product: the library's
+        x2 = x3.reshape(-1, x3.shape[-1])
+        y = (torch.nn.functional.linear(x2, w, b) if transpose else x2 @ w)
+    elif transpose:
+        y = k.linear_forward(x3, w.contiguous(),
+                             None if b is None else b.contiguous())
+    else:
+        y = k.linear_grad_input(x3, w.contiguous())
+    return y.reshape(*x.shape[:-1], n)
+
+
+class _LinearGrad(_NoSecond):
+    @staticmethod
+    def forward(dy, w, q, e, groups, wants):
+        k = _kernels(dy)
+        g = max(groups, 1)
+        dx = (_product(dy, w, groups, False) if wants[0]
+              else dy.new_empty(0))
+        dw = db = dy.new_empty(0)
+        if wants[1] or wants[2]:
+            dy3 = _groups3(dy, groups)
+            if wants[1]:
+                rows = dy3.shape[1]
+                dw = k.linear_grad_weight(
+                    dy3, q.reshape(g, rows, q.shape[-1]).contiguous(),
+                    e.reshape(g, rows, e.shape[-1]).contiguous())
+                dw = dw if groups else dw[0]
+            if wants[2]:
+                db = k.colsum(dy3)
+                db = db if groups else db[0]
+        return dx, dw, db
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, dy, w, q, e, groups, wants):
+        _refuse_nested(groups, "linear_act8")
+        n = info.batch_size
+        q, e = ((_batched(q, in_dims[2], n), _batched(e, in_dims[3], n))
+                if wants[1] else (q, e))
+        out = _LinearGrad.apply(_batched(dy, in_dims[0], n),
+                                _param_batched(w, in_dims[1]), q, e, n, wants)
+        return out, tuple(0 if want else None for want in wants)
+
+
+class _Linear8(Function):
+    # groups: as for _Norm
+
+    @staticmethod
+    def forward(x, w, b, keep, groups):
+        y = _product(x, w, groups, True, b)
+        if keep:
+            q, e = _kernels(x).act8_pack(x.contiguous())
+        else:
+            q = e = x.new_empty(0, dtype=torch.uint8)
+            e = e.clone()
+        return y, q, e
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, w, b, _, groups = inputs
+        _, q, e = output
+        ctx.mark_non_differentiable(q, e)
+        ctx.save_for_backward(w, q, e)
+        ctx.groups = groups
+        ctx.has_b = b is not None
+
+    @staticmethod
+    def backward(ctx, dy, _q, _e):
+        w, q, e = ctx.saved_tensors
+        wants = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                 ctx.has_b and ctx.needs_input_grad[2])
+        dx, dw, db = _LinearGrad.apply(dy, w, q, e, ctx.groups, wants)
+        return (dx if wants[0] else None, dw if wants[1] else None,
+                db if wants[2] else None, None, None)
+
+    @staticmethod
+    def vmap(info, in_dims, x, w, b, keep, groups):
+        _refuse_nested(groups, "linear_act8")
+        n = info.batch_size
+        x = _batched(x, in_dims[0], n)
+        if in_dims[1] is not None or in_dims[2] is not None:
+            w, b, groups = (_batched(w, in_dims[1], n),
+                            _batched(b, in_dims[2], n), n)
+        per = 0 if keep else None
+        return _Linear8.apply(x, w, b, keep, groups), (0, per, per)
+
+
+def linear_act8(x: Tensor, weight: Tensor,
+                bias: Optional[Tensor] = None) -> Tensor:
+    """``x @ weight.T + bias`` that keeps ``x`` [..., in] in 8 bits (see
+    :func:`gelu_act8`) for the weight's gradient, ``dy.T @ x8``; the values
+    held are used as they are in that product.  ``weight``: [out, in];
+    ``bias``: [out] or None.
+
+    In float32 a value that is not finite makes the results it enters NaN.
+    """
+    _check_input("x", x)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be an [out, in] tensor")
+    _check_param("weight", weight, x, (weight.shape[0], x.shape[-1]))
+    _check_param("bias", bias, x, weight.shape[:1])
+    return _Linear8.apply(x, weight, bias, _tracks(weight), 0)[0]
+
+
+__all__ = ["layer_norm", "linear_cross_entropy", "gelu_act8", "linear_act8"]

@@ -201,3 +201,157 @@ def flat_sgd_step_(theta: Tensor, delta: Tensor, lr: float) -> Tensor:
 def sanitize_(U: Tensor) -> Tensor:
     """K18 — nan_to_num on update read (reference: client.py:198)."""
     return torch.nan_to_num_(U)
+
+
+# ------------------------------------------------- token-model operators
+# Plain forms of csrc/layer_norm.hip, act8.hip and token_gemm.hip with the
+# same interface: [groups, rows, ...] inputs, parameters shared or with a
+# leading group axis, 32-bit arithmetic rounded once to the inputs' type.
+
+_ACT8_BLOCK = 128
+
+
+def _per_row(p: Optional[Tensor]) -> Optional[Tensor]:
+    """A parameter [dim] or [groups, dim] against [groups, rows, dim]."""
+    if p is None:
+        return None
+    return p.float() if p.dim() == 1 else p.float().unsqueeze(1)
+
+
+def norm_forward(x: Tensor, w: Optional[Tensor], b: Optional[Tensor],
+                 eps: float):
+    xf = x.float()
+    mean = xf.mean(-1, keepdim=True)
+    c = xf - mean
+    rstd = 1.0 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+    y = c * rstd
+    if w is not None:
+        y = y * _per_row(w)
+    if b is not None:
+        y = y + _per_row(b)
+    return y.to(x.dtype), mean.squeeze(-1), rstd.squeeze(-1)
+
+
+def norm_backward(dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor,
+                  w: Optional[Tensor], params: bool):
+    h = (x.float() - mean.unsqueeze(-1)) * rstd.unsqueeze(-1)
+    dyf = dy.float()
+    g = dyf if w is None else dyf * _per_row(w)
+    dx = rstd.unsqueeze(-1) * (g - g.mean(-1, keepdim=True)
+                               - h * (g * h).mean(-1, keepdim=True))
+    if not params:
+        empty = x.new_empty(0, x.shape[-1])
+        return dx.to(x.dtype), empty, empty.clone()
+    return (dx.to(x.dtype), (dyf * h).sum(1).to(x.dtype),
+            dyf.sum(1).to(x.dtype))
+
+
+def colsum(x: Tensor) -> Tensor:
+    return x.float().sum(1).to(x.dtype)
+
+
+def act8_pack(x: Tensor):
+    """int8 values and biased exponents (255: a block that is not finite)."""
+    n = x.shape[-1]
+    pad = (-n) % _ACT8_BLOCK
+    xf = torch.nn.functional.pad(x.float(), (0, pad))
+    blocks = xf.reshape(*x.shape[:-1], -1, _ACT8_BLOCK)
+    top = blocks.abs().amax(-1, keepdim=True)
+    finite = torch.isfinite(top)
+    m, k = torch.frexp(torch.where(finite, top, torch.ones_like(top)))
+    e = (k - 7 + (m > 127.0 / 128.0).int()).clamp(min=-126)
+    e = torch.where(top == 0, torch.full_like(e, -126), e)
+    q = torch.round(torch.ldexp(blocks, -e))
+    q = torch.where(finite, q, torch.zeros_like(q)).to(torch.int8)
+    code = torch.where(finite, e + 127, torch.full_like(e, 255))
+    return (q.reshape(*x.shape[:-1], -1)[..., :n].contiguous(),
+            code.squeeze(-1).to(torch.uint8))
+
+
+def act8_unpack(q: Tensor, e: Tensor) -> Tensor:
+    """The float32 values that 8-bit storage holds."""
+    n = q.shape[-1]
+    code = e.int().unsqueeze(-1)
+    unit = torch.ldexp(torch.ones_like(code, dtype=torch.float32),
+                       code.clamp(max=254) - 127)
+    unit = torch.where(code == 255, torch.full_like(unit, float("nan")), unit)
+    unit = unit.expand(*unit.shape[:-1], _ACT8_BLOCK)
+    return q.float() * unit.reshape(*e.shape[:-1], -1)[..., :n]
+
+
+def gelu_forward(x: Tensor, keep: bool):
+    xf = x.float()
+    y = (0.5 * xf * (1.0 + torch.erf(xf * 0.5 ** 0.5))).to(x.dtype)
+    if not keep:
+        return (y, x.new_empty(0, dtype=torch.int8),
+                x.new_empty(0, dtype=torch.uint8))
+    return (y, *act8_pack(x))
+
+
+def gelu_backward(dy: Tensor, q: Tensor, e: Tensor) -> Tensor:
+    v = act8_unpack(q, e)
+    slope = (0.5 * (1.0 + torch.erf(v * 0.5 ** 0.5))
+             + v * torch.exp(-0.5 * v * v) * 0.3989422804014327)
+    return (dy.float() * slope).to(dy.dtype)
+
+
+def linear_forward(x: Tensor, w: Tensor, b: Optional[Tensor]) -> Tensor:
+    y = torch.matmul(x.float(), w.float().transpose(-1, -2).contiguous())
+    if b is not None:
+        y = y + _per_row(b)
+    return y.to(x.dtype)
+
+
+def linear_grad_input(dy: Tensor, w: Tensor) -> Tensor:
+    return torch.matmul(dy.float(), w.float()).to(dy.dtype)
+
+
+def linear_grad_weight(dy: Tensor, q: Tensor, e: Tensor) -> Tensor:
+    dyt = dy.float().transpose(1, 2).contiguous()
+    return torch.matmul(dyt, act8_unpack(q, e)).to(dy.dtype)
+
+
+def _logits(x: Tensor, w: Tensor, bias: Optional[Tensor]) -> Tensor:
+    z = torch.matmul(x.float(), w.float().transpose(-1, -2).contiguous())
+    return z if bias is None else z + _per_row(bias)
+
+
+def loss_forward(x: Tensor, w: Tensor, target: Tensor,
+                 bias: Optional[Tensor], ignore: int, reduction: int):
+    """reduction 0: rows, 1: sum, 2: mean."""
+    vocab = w.shape[-2]
+    z = _logits(x, w, bias)
+    lse = torch.logsumexp(z, -1)
+    counted = target != ignore
+    bad = counted & ((target < 0) | (target >= vocab))
+    lse = lse.masked_fill(bad, float("nan"))
+    at = target.clamp(0, vocab - 1).unsqueeze(-1)
+    rows = torch.where(counted, lse - z.gather(-1, at).squeeze(-1),
+                       torch.zeros_like(lse))
+    count = counted.sum(-1).float()
+    if reduction == 0:
+        return rows, lse, count
+    total = rows.double().sum(-1)
+    if reduction == 2:
+        total = total / count
+    return total.float(), lse, count
+
+
+def loss_backward(grad: Tensor, x: Tensor, w: Tensor, target: Tensor,
+                  bias: Optional[Tensor], lse: Tensor, count: Tensor,
+                  ignore: int, reduction: int, want_x: bool, want_w: bool,
+                  want_b: bool):
+    z = _logits(x, w, bias)
+    p = torch.exp(z - lse.unsqueeze(-1))
+    counted = (target != ignore).unsqueeze(-1)
+    at = target.clamp(0, w.shape[-2] - 1).unsqueeze(-1)
+    p.scatter_add_(-1, at, torch.full_like(at, -1.0, dtype=p.dtype))
+    if reduction == 2:
+        grad = grad / count.unsqueeze(-1)
+    p = torch.where(counted, p * grad.unsqueeze(-1), torch.zeros_like(p))
+    none = x.new_empty(0)
+    dx = torch.matmul(p, w.float()).to(x.dtype) if want_x else none
+    dw = (torch.matmul(p.transpose(1, 2).contiguous(), x.float()).to(x.dtype)
+          if want_w else none)
+    db = p.sum(1).to(x.dtype) if want_b else none
+    return dx, dw, db

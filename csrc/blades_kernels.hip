@@ -1317,6 +1317,8 @@ torch::Tensor gram(torch::Tensor U) {
 
 }  // namespace
 
+void bind_token_ops(pybind11::module_& m);  // token_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "blades_amd CDNA4 HIP kernels (gfx950)";
   m.def("col_mean", &col_mean, "column mean (K1)");
@@ -1339,4 +1341,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "per-row squared distance to z (K6)");
   m.def("row_dots", &row_dots, "per-row dot with v (K9)");
   m.def("gram", &gram, "U U^T via f32 MFMA (K4/K8)");
+  bind_token_ops(m);
 }

@@ -1,0 +1,127 @@
+// Launch functions of the token-model operators (layer norm, linear layers
+// with a fused loss, 8-bit activation checkpoints).  Plain pointers and a
+// stream: the tensor checks live in token_bindings.cpp, the kernels in
+// layer_norm.hip, act8.hip and token_gemm.hip.
+//
+// A "group" is one client of a population trained as one batch: a group owns
+// `rows` consecutive rows and its own parameter gradients.  Parameters are
+// shared (group stride 0) or one set per group.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace token_ops {
+
+enum DType : int { kF32 = 0, kBF16 = 1 };
+
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------- layer_norm
+struct NormArgs {
+  const void* x;
+  const void* dy;     // backward only
+  const void* w;      // may be null
+  const void* b;      // may be null
+  void* y;            // forward: y, backward: dx
+  float* mean;
+  float* rstd;
+  void* dw;           // backward, may be null
+  void* db;           // backward, may be null
+  float* partial;     // backward workspace, norm_partial_floats() floats
+  long long groups, rows, dim;
+  long long w_stride, b_stride;  // elements between groups' parameters
+  float eps;
+};
+long long norm_partial_blocks(long long groups, long long rows, long long dim,
+                              DType t);
+void norm_forward(const NormArgs& a, DType t, hipStream_t s);
+void norm_backward(const NormArgs& a, DType t, hipStream_t s);
+
+// Sums over rows: out[g][c] = sum_r x[g][r][c], through a workspace of
+// groups * colsum_blocks() * cols floats.
+long long colsum_blocks(long long groups, long long rows, long long cols);
+void colsum(const void* x, void* out, float* partial, long long groups,
+            long long rows, long long cols, DType t, hipStream_t s);
+
+// ------------------------------------------------------------------- act8
+// q[rows][dim] int8 and e[rows][ceil(dim/128)]: x ~ q * 2^(e - 127).
+void act8_pack(const void* x, int8_t* q, uint8_t* e, long long rows,
+               long long dim, DType t, hipStream_t s);
+void gelu_forward(const void* x, void* y, int8_t* q, uint8_t* e,
+                  long long rows, long long dim, DType t, hipStream_t s);
+void gelu_backward(const void* dy, const int8_t* q, const uint8_t* e,
+                   void* dx, long long rows, long long dim, DType t,
+                   hipStream_t s);
+
+// ------------------------------------------------------- matrix products
+struct Mat {              // row-major, `ld` elements between rows
+  const void* p;
+  long long ld;
+  long long group;        // elements between groups (0: shared)
+  const uint8_t* e;       // exponents of 8-bit storage, else null
+  long long e_ld, e_group;
+  bool padded;            // rows may be read, as zeros, up to `ld`
+};
+
+// out[g][m][n] = sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), 32-bit sums.
+//   a_kmajor: A is stored [k][m] instead of [m][k]; likewise b_kmajor.
+// With `partial` set and splits > 1 the contraction is cut into `splits`
+// parts whose sums go to partial[split][g][m][n] and are joined afterwards;
+// `accumulate` keeps adding into `partial` (joined by the caller).
+struct Gemm {
+  Mat a, b;
+  bool a_kmajor, b_kmajor;
+  DType ta, tb;           // tb ignored where b.e is set
+  long long groups, m, n, k;
+  void* out;
+  long long out_ld, out_group;
+  DType tout;
+  const void* bias;
+  long long bias_group;
+  float* partial;
+  int splits;
+  bool accumulate;
+};
+int gemm_splits(long long groups, long long m, long long n, long long k);
+void gemm(const Gemm& g, hipStream_t s);
+// out = sum over splits of partial (+ bias), rounded to tout
+void join_partials(const float* partial, int splits, long long groups,
+                   long long m, long long n, void* out, long long out_ld,
+                   long long out_group, const void* bias,
+                   long long bias_group, DType tout, hipStream_t s);
+
+// ----------------------------------------------- loss of a linear head
+struct Loss {
+  Mat x;                  // [groups][rows][dim]
+  Mat w;                  // [groups or shared][vocab][dim]
+  const void* bias;       // [vocab], may be null
+  long long bias_group;
+  const long long* target;  // [groups][rows]
+  long long groups, rows, vocab, dim, ignore;
+  DType t;
+};
+// number of vocabulary tiles = rows of the (max, sum) partials
+long long loss_tiles(long long vocab);
+// part: [groups][tiles][rows] float2; picked: [groups][rows] float.  Writes
+// lse and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
+// group and the number of counted rows, through block_sums
+// [groups][loss_sum_blocks(rows)] double2.
+long long loss_sum_blocks(long long rows);
+void loss_forward(const Loss& l, void* part, float* picked, float* lse,
+                  float* row_loss, void* block_sums, float* loss,
+                  float* count, bool mean, hipStream_t s);
+// One piece of the vocabulary [v0, v0+nv): pt[g][v][ld] = the loss's
+// gradient in the logits, token-minor, zero beyond rows and nv up to whole
+// tiles.  grad: upstream gradient, one per group or per row.
+void loss_logit_grad(const Loss& l, long long v0, long long nv,
+                     const float* lse, const float* grad, long long grad_g,
+                     long long grad_n, const float* count, void* pt,
+                     long long pt_ld, long long pt_group, hipStream_t s);
+// out[g][v] = sum over the row of pt
+void rowsum(const void* pt, long long ld, long long group, long long groups,
+            long long rows, long long cols, void* out, long long out_group,
+            DType t, hipStream_t s);
+
+}  // namespace token_ops
