@@ -8,8 +8,9 @@
   their input in 8 bits for the backward pass.
 
 float32 and bfloat16.  GPU tensors run the HIP kernels of ``csrc/`` (and
-refuse to run without them), CPU tensors the plain forms of
-:mod:`torch_ref`.  Every operator runs under ``torch.func.grad`` and
+refuse to run without them) through dispatcher ops of the extension; CPU
+tensors run the plain forms of :mod:`torch_ref` under the autograd functions
+below, which have the same rules.  Every operator runs under ``torch.func.grad`` and
 ``torch.func.vmap`` in either nesting: a vmapped call is ONE launch over all
 clients ("groups" below), with shared or per-client parameters, and
 ``vmap(grad(...))`` gets the parameters' gradients per client from the
@@ -33,10 +34,12 @@ _DTYPES = (torch.float32, torch.bfloat16)
 _REDUCTIONS = ("none", "sum", "mean")
 
 
-def _kernels(t: Tensor):
+def _extension(x: Tensor):
+    """The HIP extension, whose ops bring their own autograd and vmap rules,
+    where ``x`` has to run on it; else None."""
     from blades_amd import ops
 
-    return ops._route(t) or _ref
+    return ops._route(x)
 
 
 # ------------------------------------------------------------------ checks
@@ -89,10 +92,15 @@ def _refuse_nested(groups: int, op: str) -> None:
 
 def _groups3(t: Tensor, groups: int) -> Tensor:
     """[groups or 1, rows, last] contiguous."""
-    lead = groups if groups else 1
-    rows = t[0].numel() // t.shape[-1] if groups and t.shape[0] else (
-        t.numel() // t.shape[-1])
-    return t.reshape(lead, rows, t.shape[-1]).contiguous()
+    g, last = max(groups, 1), t.shape[-1]
+    rows = t.numel() // (g * last) if last else 0
+    return t.reshape(g, rows, last).contiguous()
+
+
+def _groups2(t: Tensor, groups: int) -> Tensor:
+    """[groups or 1, rows] contiguous."""
+    g = max(groups, 1)
+    return t.reshape(g, t.numel() // g).contiguous()
 
 
 class _NoSecond(Function):
@@ -111,10 +119,10 @@ class _NormGrad(_NoSecond):
     @staticmethod
     def forward(dy, x, w, mean, rstd, groups, params):
         g = max(groups, 1)
-        dx, dw, db = _kernels(x).norm_backward(
+        dx, dw, db = _ref.norm_backward(
             _groups3(dy, groups), _groups3(x, groups),
-            mean.reshape(g, -1).contiguous(),
-            rstd.reshape(g, -1).contiguous(),
+            _groups2(mean, groups),
+            _groups2(rstd, groups),
             None if w is None else w.contiguous(), params)
         if not groups and params:
             dw, db = dw[0], db[0]
@@ -142,7 +150,7 @@ class _Norm(Function):
 
     @staticmethod
     def forward(x, w, b, eps, groups):
-        y, mean, rstd = _kernels(x).norm_forward(
+        y, mean, rstd = _ref.norm_forward(
             _groups3(x, groups), None if w is None else w.contiguous(),
             None if b is None else b.contiguous(), eps)
         lead = x.shape[:-1]
@@ -190,6 +198,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None,
     _check_param("bias", bias, x, x.shape[-1:])
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
+    ext = _extension(x)
+    if ext is not None:
+        return ext.layer_norm(x, weight, bias, float(eps))
     return _Norm.apply(x, weight, bias, float(eps), 0)[0]
 
 
@@ -200,11 +211,11 @@ class _HeadLossGrad(_NoSecond):
     def forward(grad, x, w, b, target, lse, count, ignore, reduction, groups,
                 wants):
         g = max(groups, 1)
-        dx, dw, db = _kernels(x).loss_backward(
-            grad.float().reshape(g, -1).contiguous(), _groups3(x, groups),
-            w.contiguous(), target.reshape(g, -1).contiguous(),
+        dx, dw, db = _ref.loss_backward(
+            _groups2(grad.float(), groups), _groups3(x, groups),
+            w.contiguous(), _groups2(target, groups),
             None if b is None else b.contiguous(),
-            lse.reshape(g, -1).contiguous(), count.reshape(g).contiguous(),
+            _groups2(lse, groups), count.reshape(g).contiguous(),
             ignore, reduction, *wants)
         if not groups:
             dw = dw[0] if wants[1] else dw
@@ -235,9 +246,9 @@ class _HeadLoss(Function):
     @staticmethod
     def forward(x, w, b, target, ignore, reduction, groups):
         g = max(groups, 1)
-        loss, lse, count = _kernels(x).loss_forward(
+        loss, lse, count = _ref.loss_forward(
             _groups3(x, groups), w.contiguous(),
-            target.reshape(g, -1).contiguous(),
+            _groups2(target, groups),
             None if b is None else b.contiguous(), ignore, reduction)
         if reduction == 0:
             loss = loss.view(target.shape)
@@ -322,6 +333,11 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got "
                          f"{reduction!r}")
+    ext = _extension(x)
+    if ext is not None:
+        return ext.linear_cross_entropy(x, weight, target, bias,
+                                        int(ignore_index),
+                                        _REDUCTIONS.index(reduction))
     return _HeadLoss.apply(x, weight, bias, target, int(ignore_index),
                            _REDUCTIONS.index(reduction), 0)[0]
 
@@ -331,7 +347,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
 class _GeluGrad(_NoSecond):
     @staticmethod
     def forward(dy, q, e):
-        return _kernels(dy).gelu_backward(dy.contiguous(), q.contiguous(),
+        return _ref.gelu_backward(dy.contiguous(), q.contiguous(),
                                           e.contiguous())
 
     @staticmethod
@@ -348,7 +364,7 @@ class _GeluGrad(_NoSecond):
 class _Gelu8(Function):
     @staticmethod
     def forward(x, keep):
-        return tuple(_kernels(x).gelu_forward(x.contiguous(), keep))
+        return tuple(_ref.gelu_forward(x.contiguous(), keep))
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -379,6 +395,9 @@ def gelu_act8(x: Tensor) -> Tensor:
     itself.
     """
     _check_input("x", x)
+    ext = _extension(x)
+    if ext is not None:
+        return ext.gelu_act8(x)
     return _Gelu8.apply(x, _tracks(x))[0]
 
 
@@ -396,26 +415,15 @@ def _tracks(t: Tensor) -> bool:
 
 def _product(x: Tensor, w: Tensor, groups: int, transpose: bool, b=None):
     """x @ w.T + b (or x @ w) with shared or per-client w."""
-    k = _kernels(x)
     x3 = _groups3(x, groups)
-    n = w.shape[-2] if transpose else w.shape[-1]
-    if (x.is_cuda and k is not _ref and w.dim() == 2
-            and x.dtype == torch.bfloat16):
-        # one plain bf16 product: the library's
-        x2 = x3.reshape(-1, x3.shape[-1])
-        y = (torch.nn.functional.linear(x2, w, b) if transpose else x2 @ w)
-    elif transpose:
-        y = k.linear_forward(x3, w.contiguous(),
-                             None if b is None else b.contiguous())
-    else:
-        y = k.linear_grad_input(x3, w.contiguous())
-    return y.reshape(*x.shape[:-1], n)
+    y = (_ref.linear_forward(x3, w, b) if transpose
+         else _ref.linear_grad_input(x3, w))
+    return y.reshape(*x.shape[:-1], y.shape[-1])
 
 
 class _LinearGrad(_NoSecond):
     @staticmethod
     def forward(dy, w, q, e, groups, wants):
-        k = _kernels(dy)
         g = max(groups, 1)
         dx = (_product(dy, w, groups, False) if wants[0]
               else dy.new_empty(0))
@@ -424,12 +432,12 @@ class _LinearGrad(_NoSecond):
             dy3 = _groups3(dy, groups)
             if wants[1]:
                 rows = dy3.shape[1]
-                dw = k.linear_grad_weight(
+                dw = _ref.linear_grad_weight(
                     dy3, q.reshape(g, rows, q.shape[-1]).contiguous(),
                     e.reshape(g, rows, e.shape[-1]).contiguous())
                 dw = dw if groups else dw[0]
             if wants[2]:
-                db = k.colsum(dy3)
+                db = _ref.colsum(dy3)
                 db = db if groups else db[0]
         return dx, dw, db
 
@@ -455,7 +463,7 @@ class _Linear8(Function):
     def forward(x, w, b, keep, groups):
         y = _product(x, w, groups, True, b)
         if keep:
-            q, e = _kernels(x).act8_pack(x.contiguous())
+            q, e = _ref.act8_pack(x.contiguous())
         else:
             q = e = x.new_empty(0, dtype=torch.uint8)
             e = e.clone()
@@ -505,6 +513,9 @@ def linear_act8(x: Tensor, weight: Tensor,
         raise ValueError("weight must be an [out, in] tensor")
     _check_param("weight", weight, x, (weight.shape[0], x.shape[-1]))
     _check_param("bias", bias, x, weight.shape[:1])
+    ext = _extension(x)
+    if ext is not None:
+        return ext.linear_act8(x, weight, bias)
     return _Linear8.apply(x, weight, bias, _tracks(weight), 0)[0]
 
 

@@ -255,7 +255,8 @@ def act8_pack(x: Tensor):
     n = x.shape[-1]
     pad = (-n) % _ACT8_BLOCK
     xf = torch.nn.functional.pad(x.float(), (0, pad))
-    blocks = xf.reshape(*x.shape[:-1], -1, _ACT8_BLOCK)
+    nb = (n + pad) // _ACT8_BLOCK
+    blocks = xf.reshape(*x.shape[:-1], nb, _ACT8_BLOCK)
     top = blocks.abs().amax(-1, keepdim=True)
     finite = torch.isfinite(top)
     m, k = torch.frexp(torch.where(finite, top, torch.ones_like(top)))
@@ -264,7 +265,7 @@ def act8_pack(x: Tensor):
     q = torch.round(torch.ldexp(blocks, -e))
     q = torch.where(finite, q, torch.zeros_like(q)).to(torch.int8)
     code = torch.where(finite, e + 127, torch.full_like(e, 255))
-    return (q.reshape(*x.shape[:-1], -1)[..., :n].contiguous(),
+    return (q.reshape(*x.shape[:-1], n + pad)[..., :n].contiguous(),
             code.squeeze(-1).to(torch.uint8))
 
 
@@ -276,7 +277,8 @@ def act8_unpack(q: Tensor, e: Tensor) -> Tensor:
                        code.clamp(max=254) - 127)
     unit = torch.where(code == 255, torch.full_like(unit, float("nan")), unit)
     unit = unit.expand(*unit.shape[:-1], _ACT8_BLOCK)
-    return q.float() * unit.reshape(*e.shape[:-1], -1)[..., :n]
+    unit = unit.reshape(*e.shape[:-1], e.shape[-1] * _ACT8_BLOCK)
+    return q.float() * unit[..., :n]
 
 
 def gelu_forward(x: Tensor, keep: bool):

@@ -1,0 +1,16 @@
+// torch's vmap headers include nlohmann/json.hpp, which torch does not ship,
+// to write their interpreters out.  Nothing here does that: declarations are
+// enough, and a call would not link.
+#pragma once
+
+#include <string>
+
+namespace nlohmann {
+struct json {
+  json();
+  template <typename T> json(const T&);
+  static json parse(const std::string&);
+  std::string dump() const;
+  template <typename T> T get() const;
+};
+}  // namespace nlohmann

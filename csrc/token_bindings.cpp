@@ -1,11 +1,21 @@
 // Tensor entry points of the token-model operators: checks, workspaces and
-// launches on the current stream of the inputs' device.  Shapes arrive
-// normalised from blades_amd/ops: contiguous [groups, rows, ...] tensors.
+// launches on the current stream of the inputs' device (contiguous
+// [groups, rows, ...] tensors), and above them the dispatcher ops with their
+// autograd and vmap rules.
 #include <torch/extension.h>
 
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/functorch/BatchedTensorImpl.h>
+#include <ATen/functorch/DynamicLayer.h>
+#include <ATen/functorch/PlumbingHelper.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/library.h>
 
 #include <limits>
 #include <optional>
@@ -536,21 +546,676 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
   return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------- dispatcher
+// The operators as torch dispatcher ops, so that autograd and the
+// torch.func transforms run without Python between the launches (a vmapped
+// forward and backward in Python costs 0.7 ms of host time, here 0.2).
+//
+//   CUDA             reshapes to [groups, rows, ...] and launches
+//   Autograd         records a node; the gradients are dispatcher ops too
+//   FuncTorchBatched moves the client axis first and calls the op on the
+//                    whole population: shared parameters stay shared,
+//                    per-client ones set `groups`
+//
+// `groups`: 0, or the number of clients on the leading axis of the inputs.
+// A gradient op called with groups gives the parameters' gradients per
+// client.
+
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+using Int3 = std::tuple<Tensor, Tensor, Tensor>;
+
+using NormSig = Int3(const Tensor&, const OptTensor&, const OptTensor&, double,
+                     int64_t);
+using NormGradSig = Int3(const Tensor&, const Tensor&, const OptTensor&,
+                         const Tensor&, const Tensor&, int64_t, bool);
+using GeluSig = Int3(const Tensor&, bool);
+using GeluGradSig = Tensor(const Tensor&, const Tensor&, const Tensor&);
+using LinearSig = Int3(const Tensor&, const Tensor&, const OptTensor&, bool,
+                       int64_t);
+using LinearGradSig = Int3(const Tensor&, const Tensor&, const Tensor&,
+                           const Tensor&, int64_t, bool, bool, bool);
+using LossSig = Int3(const Tensor&, const Tensor&, const Tensor&,
+                     const OptTensor&, int64_t, int64_t, int64_t);
+using LossGradSig = Int3(const Tensor&, const Tensor&, const Tensor&,
+                         const Tensor&, const OptTensor&, const Tensor&,
+                         const Tensor&, int64_t, int64_t, int64_t, bool, bool,
+                         bool);
+
+template <typename Sig>
+c10::TypedOperatorHandle<Sig> find_op(const char* name) {
+  return c10::Dispatcher::singleton()
+      .findSchemaOrThrow(name, "")
+      .typed<Sig>();
+}
+#define BLADES_OP(fn, name, Sig)                                      \
+  const c10::TypedOperatorHandle<Sig>& fn() {                         \
+    static const auto op = find_op<Sig>("blades_amd::" name);         \
+    return op;                                                        \
+  }
+BLADES_OP(norm_op, "layer_norm", NormSig)
+BLADES_OP(norm_grad_op, "layer_norm_grad", NormGradSig)
+BLADES_OP(gelu_op, "gelu_act8", GeluSig)
+BLADES_OP(gelu_grad_op, "gelu_act8_grad", GeluGradSig)
+BLADES_OP(linear_op, "linear_act8", LinearSig)
+BLADES_OP(linear_grad_op, "linear_act8_grad", LinearGradSig)
+BLADES_OP(loss_op, "linear_cross_entropy", LossSig)
+BLADES_OP(loss_grad_op, "linear_cross_entropy_grad", LossGradSig)
+#undef BLADES_OP
+
+// ------------------------------------------------------------ CUDA kernels
+
+OptTensor contig(const OptTensor& t) {
+  return t.has_value() && t->defined() ? OptTensor(t->contiguous())
+                                       : OptTensor();
+}
+
+// [groups or 1, rows, last] contiguous
+Tensor groups3(const Tensor& t, int64_t groups) {
+  const int64_t g = groups ? groups : 1, last = t.size(-1);
+  return t.reshape({g, last ? t.numel() / (g * last) : 0, last}).contiguous();
+}
+// [groups or 1, rows] contiguous
+Tensor groups2(const Tensor& t, int64_t groups) {
+  const int64_t g = groups ? groups : 1;
+  return t.reshape({g, t.numel() / g}).contiguous();
+}
+Tensor ungroup(const Tensor& t, int64_t groups, bool have) {
+  return groups || !have ? t : t.select(0, 0);
+}
+
+Int3 norm_cuda(const Tensor& x, const OptTensor& w, const OptTensor& b,
+               double eps, int64_t groups) {
+  auto [y, mean, rstd] =
+      norm_forward_t(groups3(x, groups), contig(w), contig(b), eps);
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  return {y.view(x.sizes()), mean.view(lead), rstd.view(lead)};
+}
+
+Int3 norm_grad_cuda(const Tensor& dy, const Tensor& x, const OptTensor& w,
+                    const Tensor& mean, const Tensor& rstd, int64_t groups,
+                    bool params) {
+  auto [dx, dw, db] = norm_backward_t(
+      groups3(dy, groups), groups3(x, groups), groups2(mean, groups),
+      groups2(rstd, groups), contig(w), params);
+  return {dx.view(x.sizes()), ungroup(dw, groups, params),
+          ungroup(db, groups, params)};
+}
+
+Int3 gelu_cuda(const Tensor& x, bool keep) {
+  return gelu_forward_t(x.contiguous(), keep);
+}
+Tensor gelu_grad_cuda(const Tensor& dy, const Tensor& q, const Tensor& e) {
+  return gelu_backward_t(dy.contiguous(), q.contiguous(), e.contiguous());
+}
+
+// One plain bf16 product is the library's; fp32 and per-client products run
+// the kernels of token_gemm.hip.
+bool plain_product(const Tensor& x, const Tensor& w) {
+  return w.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.numel() > 0;
+}
+
+Int3 linear_cuda(const Tensor& x, const Tensor& w, const OptTensor& b,
+                 bool keep, int64_t groups) {
+  c10::DeviceGuard guard(x.device());
+  Tensor y;
+  auto shape = x.sizes().vec();
+  shape.back() = w.size(-2);
+  if (plain_product(x, w) && (!b.has_value() || b->dim() == 1)) {
+    const Tensor x2 = x.reshape({-1, x.size(-1)}), wt = w.t();
+    y = b.has_value() ? at::addmm(*b, x2, wt) : at::mm(x2, wt);
+  } else {
+    y = linear_forward_t(groups3(x, groups), w.contiguous(), contig(b));
+  }
+  Tensor q, e;
+  if (keep) {
+    std::tie(q, e) = act8_pack_t(x.contiguous());
+  } else {
+    q = at::empty({0}, x.options().dtype(at::kChar));
+    e = at::empty({0}, x.options().dtype(at::kByte));
+  }
+  return {y.view(shape), q, e};
+}
+
+Int3 linear_grad_cuda(const Tensor& dy, const Tensor& w, const Tensor& q,
+                      const Tensor& e, int64_t groups, bool want_x,
+                      bool want_w, bool want_b) {
+  c10::DeviceGuard guard(dy.device());
+  const Tensor dy3 = groups3(dy, groups);
+  Tensor dx, dw, db;
+  dx = dw = db = at::empty({0}, dy.options());
+  if (want_x) {
+    auto shape = dy.sizes().vec();
+    shape.back() = w.size(-1);
+    dx = (plain_product(dy, w)
+              ? at::mm(dy3.view({-1, dy.size(-1)}), w)
+              : linear_grad_input_t(dy3, w.contiguous())).view(shape);
+  }
+  if (want_w)
+    dw = ungroup(linear_grad_weight_t(dy3, groups3(q, groups),
+                                      groups3(e, groups)), groups, true);
+  if (want_b) db = ungroup(colsum_t(dy3), groups, true);
+  return {dx, dw, db};
+}
+
+Int3 loss_cuda(const Tensor& x, const Tensor& w, const Tensor& target,
+               const OptTensor& b, int64_t ignore, int64_t reduction,
+               int64_t groups) {
+  auto [loss, lse, count] =
+      loss_forward_t(groups3(x, groups), w.contiguous(),
+                     groups2(target, groups), contig(b), ignore, reduction);
+  if (reduction == 0)
+    loss = loss.view(target.sizes());
+  else
+    loss = ungroup(loss, groups, true);
+  return {loss, lse.view(target.sizes()), ungroup(count, groups, true)};
+}
+
+Int3 loss_grad_cuda(const Tensor& grad, const Tensor& x, const Tensor& w,
+                    const Tensor& target, const OptTensor& b,
+                    const Tensor& lse, const Tensor& count, int64_t ignore,
+                    int64_t reduction, int64_t groups, bool want_x,
+                    bool want_w, bool want_b) {
+  auto [dx, dw, db] = loss_backward_t(
+      groups2(grad, groups).to(at::kFloat), groups3(x, groups),
+      w.contiguous(), groups2(target, groups), contig(b),
+      groups2(lse, groups), groups2(count, groups), ignore, reduction, want_x,
+      want_w, want_b);
+  return {want_x ? dx.view(x.sizes()) : dx, ungroup(dw, groups, want_w),
+          ungroup(db, groups, want_b)};
+}
+
+// ---------------------------------------------------------------- autograd
+
+Tensor or_undefined(const OptTensor& t) {
+  return t.has_value() ? *t : Tensor();
+}
+OptTensor or_none(const Tensor& t) {
+  return t.defined() ? OptTensor(t) : OptTensor();
+}
+
+// Base of the nodes: tensors to keep, released together.
+struct TokenNode : public Node {
+  std::vector<SavedVariable> saved;
+  void keep(std::initializer_list<Tensor> ts) {
+    for (const Tensor& t : ts) saved.emplace_back(t, false);
+  }
+  Tensor get(size_t i) { return saved[i].unpack(); }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : saved) s.reset_data();
+  }
+  variable_list none(size_t n) { return variable_list(n); }
+};
+
+struct NormNode : public TokenNode {            // x, w, mean, rstd
+  int64_t groups = 0;
+  std::string name() const override { return "LayerNormBackward"; }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return none(3);
+    const bool want_w = task_should_compute_output(1);
+    const bool want_b = task_should_compute_output(2);
+    auto [dx, dw, db] =
+        norm_grad_op().call(grads[0], get(0), or_none(get(1)), get(2), get(3),
+                            groups, want_w || want_b);
+    return {dx, want_w ? dw : Tensor(), want_b ? db : Tensor()};
+  }
+};
+
+struct GeluNode : public TokenNode {            // q, e
+  std::string name() const override { return "GeluAct8Backward"; }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return none(1);
+    return {gelu_grad_op().call(grads[0], get(0), get(1))};
+  }
+};
+
+struct LinearNode : public TokenNode {          // w, q, e
+  int64_t groups = 0;
+  std::string name() const override { return "LinearAct8Backward"; }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return none(3);
+    const bool want[3] = {task_should_compute_output(0),
+                          task_should_compute_output(1),
+                          task_should_compute_output(2)};
+    auto [dx, dw, db] =
+        linear_grad_op().call(grads[0], get(0), get(1), get(2), groups,
+                              want[0], want[1], want[2]);
+    return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
+            want[2] ? db : Tensor()};
+  }
+};
+
+struct LossNode : public TokenNode {            // x, w, target, b, lse, count
+  int64_t ignore = 0, reduction = 0, groups = 0;
+  std::string name() const override { return "LinearCrossEntropyBackward"; }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return none(3);
+    const bool want[3] = {task_should_compute_output(0),
+                          task_should_compute_output(1),
+                          task_should_compute_output(2)};
+    Tensor grad = grads[0], w = get(1), target = get(2), count = get(5);
+    int64_t red = reduction, g = groups;
+    if (g && w.dim() == 2) {
+      // shared parameters: one sum over all clients' rows, each row with its
+      // client's share of the upstream gradient
+      if (red == 2) grad = grad / count;
+      if (red != 0) {
+        std::vector<int64_t> ones(target.dim(), 1);
+        ones[0] = -1;
+        grad = grad.reshape(ones).expand(target.sizes());
+      }
+      red = 0;
+      g = 0;
+      count = count.narrow(0, 0, 1);
+    }
+    auto [dx, dw, db] =
+        loss_grad_op().call(grad, get(0), w, target, or_none(get(3)), get(4),
+                            count, ignore, red, g, want[0], want[1], want[2]);
+    return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
+            want[2] ? db : Tensor()};
+  }
+};
+
+template <typename N>
+std::shared_ptr<N> make_node(torch::autograd::edge_list&& edges) {
+  std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
+  n->set_next_edges(std::move(edges));
+  return n;
+}
+
+Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
+                   const OptTensor& b, double eps, int64_t groups) {
+  std::shared_ptr<NormNode> node;
+  const Tensor wt = or_undefined(w), bt = or_undefined(b);
+  if (torch::autograd::compute_requires_grad(x, wt, bt))
+    node = make_node<NormNode>(torch::autograd::collect_next_edges(x, wt, bt));
+  Int3 out;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out = norm_op().redispatch(ks & c10::after_autograd_keyset, x, w, b, eps,
+                               groups);
+  }
+  if (node) {
+    node->groups = groups;
+    node->keep({x, wt, std::get<1>(out), std::get<2>(out)});
+    torch::autograd::set_history(std::get<0>(out), node);
+  }
+  return out;
+}
+
+// `keep` is set by the first level that needs the 8-bit input; a level below
+// it (the call on a vmap's whole population) must not drop it.
+Int3 gelu_autograd(c10::DispatchKeySet ks, const Tensor& x, bool keep) {
+  std::shared_ptr<GeluNode> node;
+  if (torch::autograd::compute_requires_grad(x))
+    node = make_node<GeluNode>(torch::autograd::collect_next_edges(x));
+  Int3 out;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out = gelu_op().redispatch(ks & c10::after_autograd_keyset, x,
+                               keep || node != nullptr);
+  }
+  if (node) {
+    node->keep({std::get<1>(out), std::get<2>(out)});
+    torch::autograd::set_history(std::get<0>(out), node);
+  }
+  return out;
+}
+
+Int3 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
+                     const OptTensor& b, bool keep, int64_t groups) {
+  std::shared_ptr<LinearNode> node;
+  const Tensor bt = or_undefined(b);
+  if (torch::autograd::compute_requires_grad(x, w, bt))
+    node =
+        make_node<LinearNode>(torch::autograd::collect_next_edges(x, w, bt));
+  Int3 out;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out = linear_op().redispatch(
+        ks & c10::after_autograd_keyset, x, w, b,
+        keep || torch::autograd::compute_requires_grad(w), groups);
+  }
+  if (node) {
+    node->groups = groups;
+    node->keep({w, std::get<1>(out), std::get<2>(out)});
+    torch::autograd::set_history(std::get<0>(out), node);
+  }
+  return out;
+}
+
+Int3 loss_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
+                   const Tensor& target, const OptTensor& b, int64_t ignore,
+                   int64_t reduction, int64_t groups) {
+  std::shared_ptr<LossNode> node;
+  const Tensor bt = or_undefined(b);
+  if (torch::autograd::compute_requires_grad(x, w, bt))
+    node = make_node<LossNode>(torch::autograd::collect_next_edges(x, w, bt));
+  Int3 out;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out = loss_op().redispatch(ks & c10::after_autograd_keyset, x, w, target,
+                               b, ignore, reduction, groups);
+  }
+  if (node) {
+    node->ignore = ignore;
+    node->reduction = reduction;
+    node->groups = groups;
+    node->keep({x, w, target, bt, std::get<1>(out), std::get<2>(out)});
+    torch::autograd::set_history(std::get<0>(out), node);
+  }
+  return out;
+}
+
+// The gradients are not differentiable again: asking for it raises.
+template <typename... T>
+std::shared_ptr<Node> refuse_second(const char* op, const T&... inputs) {
+  if (!torch::autograd::compute_requires_grad(inputs...)) return nullptr;
+  std::shared_ptr<Node> n(new torch::autograd::NotImplemented(op),
+                          torch::autograd::deleteNode);
+  n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return n;
+}
+
+Int3 with_history(Int3 out, const std::shared_ptr<Node>& n) {
+  if (n) {
+    torch::autograd::set_history(std::get<0>(out), n);
+    torch::autograd::set_history(std::get<1>(out), n);
+    torch::autograd::set_history(std::get<2>(out), n);
+  }
+  return out;
+}
+
+Int3 norm_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
+                        const Tensor& x, const OptTensor& w,
+                        const Tensor& mean, const Tensor& rstd, int64_t groups,
+                        bool params) {
+  auto n = refuse_second("layer_norm's gradient", dy, x, or_undefined(w));
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return with_history(
+      norm_grad_op().redispatch(ks & c10::after_autograd_keyset, dy, x, w,
+                                mean, rstd, groups, params), n);
+}
+
+Tensor gelu_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
+                          const Tensor& q, const Tensor& e) {
+  auto n = refuse_second("gelu_act8's gradient", dy);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor out =
+      gelu_grad_op().redispatch(ks & c10::after_autograd_keyset, dy, q, e);
+  if (n) torch::autograd::set_history(out, n);
+  return out;
+}
+
+Int3 linear_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
+                          const Tensor& w, const Tensor& q, const Tensor& e,
+                          int64_t groups, bool wx, bool ww, bool wb) {
+  auto n = refuse_second("linear_act8's gradient", dy, w);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return with_history(
+      linear_grad_op().redispatch(ks & c10::after_autograd_keyset, dy, w, q, e,
+                                  groups, wx, ww, wb), n);
+}
+
+Int3 loss_grad_autograd(c10::DispatchKeySet ks, const Tensor& grad,
+                        const Tensor& x, const Tensor& w, const Tensor& target,
+                        const OptTensor& b, const Tensor& lse,
+                        const Tensor& count, int64_t ignore, int64_t reduction,
+                        int64_t groups, bool wx, bool ww, bool wb) {
+  auto n = refuse_second("linear_cross_entropy's gradient", grad, x, w,
+                         or_undefined(b));
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return with_history(
+      loss_grad_op().redispatch(ks & c10::after_autograd_keyset, grad, x, w,
+                                target, b, lse, count, ignore, reduction,
+                                groups, wx, ww, wb), n);
+}
+
+// -------------------------------------------------------------------- vmap
+
+namespace fn = at::functorch;
+using Dim = std::optional<int64_t>;
+
+// The vmap level being processed; its key stays off while it lives.
+struct Level {
+  c10::impl::ExcludeDispatchKeyGuard guard{
+      c10::DispatchKey::FuncTorchBatched};
+  int64_t level, size;
+  Level() {
+    const auto layer = fn::maybeCurrentDynamicLayer();
+    TORCH_CHECK(layer.has_value(), "a batched tensor escaped its vmap");
+    level = layer->layerId();
+    size = layer->batchSize().guard_int(__FILE__, __LINE__);
+  }
+  Tensor open(const Tensor& t, Dim& d) const {
+    if (!t.defined()) return t;
+    auto [v, dim] = fn::unwrapTensorAtLevel(t, level);
+    d = dim;
+    return v;
+  }
+  // client axis first; a tensor without one is repeated
+  Tensor all(const Tensor& t) const {
+    Dim d;
+    Tensor v = open(t, d);
+    if (!v.defined()) return v;
+    if (d) return v.movedim(*d, 0);
+    auto shape = v.sizes().vec();
+    shape.insert(shape.begin(), size);
+    return v.unsqueeze(0).expand(shape);
+  }
+  OptTensor all(const OptTensor& t) const {
+    return t.has_value() ? OptTensor(all(*t)) : t;
+  }
+  // client axis first, or left shared
+  Tensor param(const Tensor& t) const {
+    Dim d;
+    Tensor v = open(t, d);
+    return v.defined() && d ? v.movedim(*d, 0) : v;
+  }
+  OptTensor param(const OptTensor& t) const {
+    return t.has_value() ? OptTensor(param(*t)) : t;
+  }
+  bool has(const Tensor& t) const {
+    return t.defined() && fn::isBatchedAtLevel(t, level);
+  }
+  bool has(const OptTensor& t) const { return t.has_value() && has(*t); }
+  Tensor close(const Tensor& t, bool batched = true) const {
+    return batched ? fn::makeBatched(t, 0, level) : t;
+  }
+  Int3 close(const Int3& t, bool a, bool b, bool c) const {
+    return {close(std::get<0>(t), a), close(std::get<1>(t), b),
+            close(std::get<2>(t), c)};
+  }
+};
+
+void refuse_nested(int64_t groups, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      groups == 0, op,
+      ": a vmap over clients inside another vmap is not supported");
+}
+
+Int3 norm_vmap(const Tensor& x, const OptTensor& w, const OptTensor& b,
+               double eps, int64_t groups) {
+  Level v;
+  if (!v.has(x) && !v.has(w) && !v.has(b))
+    return norm_op().call(x, w, b, eps, groups);
+  refuse_nested(groups, "layer_norm");
+  const bool own = v.has(w) || v.has(b);
+  return v.close(
+      norm_op().call(v.all(x), own ? v.all(w) : w, own ? v.all(b) : b, eps,
+                     own ? v.size : 0), true, true, true);
+}
+
+Int3 norm_grad_vmap(const Tensor& dy, const Tensor& x, const OptTensor& w,
+                    const Tensor& mean, const Tensor& rstd, int64_t groups,
+                    bool params) {
+  Level v;
+  if (!v.has(dy) && !v.has(x) && !v.has(w) && !v.has(mean) && !v.has(rstd))
+    return norm_grad_op().call(dy, x, w, mean, rstd, groups, params);
+  refuse_nested(groups, "layer_norm");
+  return v.close(
+      norm_grad_op().call(v.all(dy), v.all(x), v.param(w), v.all(mean),
+                          v.all(rstd), v.size, params), true, params, params);
+}
+
+Int3 gelu_vmap(const Tensor& x, bool keep) {
+  Level v;
+  if (!v.has(x)) return gelu_op().call(x, keep);
+  Int3 out = gelu_op().call(v.all(x), keep);
+  const bool kept = std::get<1>(out).numel() == std::get<0>(out).numel();
+  return v.close(out, true, kept, kept);
+}
+
+Tensor gelu_grad_vmap(const Tensor& dy, const Tensor& q, const Tensor& e) {
+  Level v;
+  if (!v.has(dy) && !v.has(q) && !v.has(e))
+    return gelu_grad_op().call(dy, q, e);
+  return v.close(gelu_grad_op().call(v.all(dy), v.all(q), v.all(e)));
+}
+
+Int3 linear_vmap(const Tensor& x, const Tensor& w, const OptTensor& b,
+                 bool keep, int64_t groups) {
+  Level v;
+  if (!v.has(x) && !v.has(w) && !v.has(b))
+    return linear_op().call(x, w, b, keep, groups);
+  refuse_nested(groups, "linear_act8");
+  const bool own = v.has(w) || v.has(b);
+  const Tensor xa = v.all(x);
+  Int3 out = linear_op().call(xa, own ? v.all(w) : w, own ? v.all(b) : b, keep,
+                              own ? v.size : 0);
+  const bool kept = std::get<1>(out).dim() == xa.dim();
+  return v.close(out, true, kept, kept);
+}
+
+Int3 linear_grad_vmap(const Tensor& dy, const Tensor& w, const Tensor& q,
+                      const Tensor& e, int64_t groups, bool wx, bool ww,
+                      bool wb) {
+  Level v;
+  if (!v.has(dy) && !v.has(w) && !v.has(q) && !v.has(e))
+    return linear_grad_op().call(dy, w, q, e, groups, wx, ww, wb);
+  refuse_nested(groups, "linear_act8");
+  return v.close(
+      linear_grad_op().call(v.all(dy), v.param(w), ww ? v.all(q) : q,
+                            ww ? v.all(e) : e, v.size, wx, ww, wb),
+      wx, ww, wb);
+}
+
+Int3 loss_vmap(const Tensor& x, const Tensor& w, const Tensor& target,
+               const OptTensor& b, int64_t ignore, int64_t reduction,
+               int64_t groups) {
+  Level v;
+  if (!v.has(x) && !v.has(w) && !v.has(target) && !v.has(b))
+    return loss_op().call(x, w, target, b, ignore, reduction, groups);
+  refuse_nested(groups, "linear_cross_entropy");
+  const bool own = v.has(w) || v.has(b);
+  return v.close(
+      loss_op().call(v.all(x), own ? v.all(w) : w, v.all(target),
+                     own ? v.all(b) : b, ignore, reduction, v.size),
+      true, true, true);
+}
+
+Int3 loss_grad_vmap(const Tensor& grad, const Tensor& x, const Tensor& w,
+                    const Tensor& target, const OptTensor& b,
+                    const Tensor& lse, const Tensor& count, int64_t ignore,
+                    int64_t reduction, int64_t groups, bool wx, bool ww,
+                    bool wb) {
+  Level v;
+  if (!v.has(grad) && !v.has(x) && !v.has(w) && !v.has(target) && !v.has(b)
+      && !v.has(lse) && !v.has(count))
+    return loss_grad_op().call(grad, x, w, target, b, lse, count, ignore,
+                               reduction, groups, wx, ww, wb);
+  refuse_nested(groups, "linear_cross_entropy");
+  return v.close(
+      loss_grad_op().call(v.all(grad), v.all(x), v.param(w), v.all(target),
+                          v.param(b), v.all(lse), v.all(count), ignore,
+                          reduction, v.size, wx, ww, wb), wx, ww, wb);
+}
+
+// ------------------------------------------------------------ entry points
+
+Tensor layer_norm_py(const Tensor& x, const OptTensor& w, const OptTensor& b,
+                     double eps) {
+  return std::get<0>(norm_op().call(x, w, b, eps, 0));
+}
+Tensor gelu_act8_py(const Tensor& x) {
+  return std::get<0>(gelu_op().call(x, false));
+}
+Tensor linear_act8_py(const Tensor& x, const Tensor& w, const OptTensor& b) {
+  return std::get<0>(linear_op().call(x, w, b, false, 0));
+}
+Tensor linear_cross_entropy_py(const Tensor& x, const Tensor& w,
+                               const Tensor& target, const OptTensor& b,
+                               int64_t ignore, int64_t reduction) {
+  return std::get<0>(loss_op().call(x, w, target, b, ignore, reduction, 0));
+}
+
 }  // namespace
 
+TORCH_LIBRARY(blades_amd, m) {
+  m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, int groups) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("layer_norm_grad(Tensor dy, Tensor x, Tensor? w, Tensor mean, "
+        "Tensor rstd, int groups, bool params) -> (Tensor, Tensor, Tensor)");
+  m.def("gelu_act8(Tensor x, bool keep) -> (Tensor, Tensor, Tensor)");
+  m.def("gelu_act8_grad(Tensor dy, Tensor q, Tensor e) -> Tensor");
+  m.def("linear_act8(Tensor x, Tensor w, Tensor? b, bool keep, int groups) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("linear_act8_grad(Tensor dy, Tensor w, Tensor q, Tensor e, "
+        "int groups, bool want_x, bool want_w, bool want_b) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy(Tensor x, Tensor w, Tensor target, Tensor? b, "
+        "int ignore, int reduction, int groups) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy_grad(Tensor grad, Tensor x, Tensor w, "
+        "Tensor target, Tensor? b, Tensor lse, Tensor count, int ignore, "
+        "int reduction, int groups, bool want_x, bool want_w, bool want_b) "
+        "-> (Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(blades_amd, CUDA, m) {
+  m.impl("layer_norm", TORCH_FN(norm_cuda));
+  m.impl("layer_norm_grad", TORCH_FN(norm_grad_cuda));
+  m.impl("gelu_act8", TORCH_FN(gelu_cuda));
+  m.impl("gelu_act8_grad", TORCH_FN(gelu_grad_cuda));
+  m.impl("linear_act8", TORCH_FN(linear_cuda));
+  m.impl("linear_act8_grad", TORCH_FN(linear_grad_cuda));
+  m.impl("linear_cross_entropy", TORCH_FN(loss_cuda));
+  m.impl("linear_cross_entropy_grad", TORCH_FN(loss_grad_cuda));
+}
+
+TORCH_LIBRARY_IMPL(blades_amd, Autograd, m) {
+  m.impl("layer_norm", TORCH_FN(norm_autograd));
+  m.impl("layer_norm_grad", TORCH_FN(norm_grad_autograd));
+  m.impl("gelu_act8", TORCH_FN(gelu_autograd));
+  m.impl("gelu_act8_grad", TORCH_FN(gelu_grad_autograd));
+  m.impl("linear_act8", TORCH_FN(linear_autograd));
+  m.impl("linear_act8_grad", TORCH_FN(linear_grad_autograd));
+  m.impl("linear_cross_entropy", TORCH_FN(loss_autograd));
+  m.impl("linear_cross_entropy_grad", TORCH_FN(loss_grad_autograd));
+}
+
+TORCH_LIBRARY_IMPL(blades_amd, FuncTorchBatched, m) {
+  m.impl("layer_norm", TORCH_FN(norm_vmap));
+  m.impl("layer_norm_grad", TORCH_FN(norm_grad_vmap));
+  m.impl("gelu_act8", TORCH_FN(gelu_vmap));
+  m.impl("gelu_act8_grad", TORCH_FN(gelu_grad_vmap));
+  m.impl("linear_act8", TORCH_FN(linear_vmap));
+  m.impl("linear_act8_grad", TORCH_FN(linear_grad_vmap));
+  m.impl("linear_cross_entropy", TORCH_FN(loss_vmap));
+  m.impl("linear_cross_entropy_grad", TORCH_FN(loss_grad_vmap));
+}
+
 void bind_token_ops(pybind11::module_& m) {
-  m.def("norm_forward", &norm_forward_t, "layer norm with its statistics");
-  m.def("norm_backward", &norm_backward_t, "layer norm gradients per group");
-  m.def("colsum", &colsum_t, "sum over rows per group");
-  m.def("act8_pack", &act8_pack_t, "activations to 8-bit storage");
-  m.def("gelu_forward", &gelu_forward_t, "GELU, keeping its input in 8 bits");
-  m.def("gelu_backward", &gelu_backward_t, "GELU gradient from 8-bit input");
-  m.def("linear_forward", &linear_forward_t, "x w' + b per group");
-  m.def("linear_grad_input", &linear_grad_input_t, "dy w per group");
-  m.def("linear_grad_weight", &linear_grad_weight_t,
-        "dy' x per group, x in 8-bit storage");
-  m.def("loss_forward", &loss_forward_t,
+  using nogil = py::call_guard<py::gil_scoped_release>;
+  m.def("layer_norm", &layer_norm_py, nogil(), "layer norm");
+  m.def("gelu_act8", &gelu_act8_py, nogil(), "GELU, its input kept in 8 bits");
+  m.def("linear_act8", &linear_act8_py, nogil(),
+        "linear layer, its input kept in 8 bits");
+  m.def("linear_cross_entropy", &linear_cross_entropy_py, nogil(),
         "cross entropy of a linear head without its logits");
-  m.def("loss_backward", &loss_backward_t,
-        "gradients of that loss, in pieces of the vocabulary");
 }

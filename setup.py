@@ -23,6 +23,8 @@ setup(
             sources=["csrc/blades_kernels.hip", "csrc/token_bindings.cpp",
                      "csrc/layer_norm.hip", "csrc/act8.hip",
                      "csrc/token_gemm.hip"],
+            include_dirs=[os.path.join(os.path.dirname(
+                os.path.abspath(__file__)), "csrc", "compat")],
             depends=["csrc/token_ops.h", "csrc/token_device.h"],
             extra_compile_args={
                 "cxx": ["-O3"],

@@ -1,0 +1,895 @@
+"""Token-model training operators against plain forms in 64 bits.
+
+Tolerances are bounds, not fits.  u is half a step of the outputs' type
+(2^-8 bf16, 2^-24 fp32), U = 2^-24 the kernels' arithmetic.  A sum of n
+products carries at most (n + 8) U times the sum of the products' magnitudes
+(n - 1 additions, the products' and the operands' roundings, and slack for
+the order), and the output one rounding more.
+"""
+import math
+
+import pytest
+import torch
+
+from blades_amd import ops
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+DTYPES = [torch.float32, torch.bfloat16]
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+gpu = pytest.mark.gpu
+
+
+def rand(*shape, dtype=torch.float32, device="cpu", seed=0, scale=1.0,
+         shift=0.0):
+    g = torch.Generator().manual_seed(seed + sum(shape))
+    t = torch.randn(*shape, generator=g) * scale + shift
+    return t.to(dtype).to(device)
+
+
+def near(got, want, bound, name=""):
+    """|got - want| <= bound elementwise; NaN only where wanted."""
+    got, want = got.double().cpu(), want.double().cpu()
+    bound = torch.as_tensor(bound, dtype=torch.float64).cpu()
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    assert torch.equal(got.isnan(), want.isnan()), name
+    over = ((got - want).abs() - bound).nan_to_num(nan=0.0, posinf=math.inf)
+    same = got == want                                   # infinities
+    over = torch.where(same, torch.zeros_like(over), over)
+    if over.numel():
+        assert over.max() <= 0, (name, float(over.max()),
+                                 float((got - want).abs().max()))
+
+
+# ------------------------------------------------------------- definitions
+
+def norm64(x, w, b, dy, eps):
+    """y, dx, dw, db and bounds on their errors in units of U."""
+    x, dy = x.double(), dy.double()
+    n = x.shape[-1]
+    w = torch.ones(n, dtype=x.dtype, device=x.device) if w is None \
+        else w.double()
+    mean = x.mean(-1, keepdim=True)
+    c = x - mean
+    var = (c * c).mean(-1, keepdim=True)
+    r = 1 / (var + eps).sqrt()
+    h = c * r
+    y = h * w + (0 if b is None else b.double())
+    g = dy * w
+    dx = r * (g - g.mean(-1, keepdim=True)
+              - h * (g * h).mean(-1, keepdim=True))
+    flat = (-1, n)
+    dw = (dy * h).reshape(flat).sum(0)
+    db = dy.reshape(flat).sum(0)
+    # mean: (n + 8) U mean|x|; rstd: relative (n + 8) U plus what an error of
+    # the mean does to h
+    k = n + 8
+    em = k * x.abs().mean(-1, keepdim=True)
+    eh = r * (em + c.abs() + x.abs()) + k * h.abs()
+    ey = eh * w.abs() + 4 * y.abs()
+    gm = g.abs().mean(-1, keepdim=True)
+    ghm = (g * h).abs().mean(-1, keepdim=True)
+    ehm = (g.abs() * eh).mean(-1, keepdim=True)
+    ex = r * (k * (g.abs() + gm + h.abs() * ghm) + eh * ghm
+              + h.abs() * ehm) + k * dx.abs()
+    rows = max(1, x.numel() // n)
+    ew = ((rows + 8) * (dy * h).abs() + dy.abs() * eh).reshape(flat).sum(0)
+    eb = (rows + 8) * dy.abs().reshape(flat).sum(0)
+    return (y, dx, dw, db), (ey, ex, ew, eb)
+
+
+def stored64(x):
+    """What 8-bit storage holds of x, by search for the exponent."""
+    x = x.double()
+    out = torch.empty_like(x)
+    n = x.shape[-1]
+    for lo in range(0, n, 128):
+        part = x[..., lo:lo + 128]
+        top = part.abs().amax(-1, keepdim=True)
+        e = torch.full_like(top, -126.0)
+        for _ in range(300):
+            e = torch.where(127.0 * torch.exp2(e) < top, e + 1, e)
+            if bool((127.0 * torch.exp2(e) >= top).logical_or(
+                    ~torch.isfinite(top)).all()):
+                break
+        unit = torch.exp2(e)
+        v = torch.round(part / unit) * unit
+        out[..., lo:lo + 128] = torch.where(torch.isfinite(top), v,
+                                            torch.full_like(v, math.nan))
+    return out
+
+
+def gelu64(x):
+    x = x.double()
+    return x * 0.5 * torch.erfc(-x / math.sqrt(2))
+
+
+def gelu_slope64(v):
+    return (0.5 * torch.erfc(-v / math.sqrt(2))
+            + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi))
+
+
+def loss64(x, w, y, b, ignore):
+    """Row losses and lse [rows]."""
+    z = x.double() @ w.double().t()
+    if b is not None:
+        z = z + b.double()
+    lse = torch.logsumexp(z, -1)
+    keep = y != ignore
+    at = y.clamp(0, w.shape[0] - 1)
+    rows = lse - z.gather(1, at[:, None])[:, 0]
+    return torch.where(keep, rows, torch.zeros_like(rows)), lse, z
+
+
+def loss_grads64(x, w, y, b, ignore, row_grad):
+    rows, lse, z = loss64(x, w, y, b, ignore)
+    p = torch.exp(z - lse[:, None])
+    at = y.clamp(0, w.shape[0] - 1)
+    p[torch.arange(len(y)), at] -= 1
+    p = torch.where((y != ignore)[:, None], p * row_grad[:, None],
+                    torch.zeros_like(p))
+    return p @ w.double(), p.t() @ x.double(), p.sum(0), p
+
+
+# -------------------------------------------------------------- layer norm
+
+NORM_SHAPES = [(1, 1), (3, 2), (7, 16), (33, 64), (130, 65), (64, 128),
+               (50, 300), (5, 512), (9, 1000), (3, 1024), (300, 2048),
+               (2, 2050), (17, 4096), (2, 5001), (3, 8192), (2, 16384),
+               (1, 20001)]
+
+
+def check_norm(x, w, b, dy, eps=1e-5):
+    dtype = x.dtype
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)
+              if t is not None]
+    it = iter(leaves)
+    xl, wl, bl = (next(it) if t is not None else None for t in (x, w, b))
+    y = ops.layer_norm(xl, wl, bl, eps)
+    grads = torch.autograd.grad(y, leaves, dy)
+    want, err = norm64(x, w, b, dy, eps)
+    got = [y, grads[0], grads[1] if w is not None else None,
+           grads[-1] if b is not None else None]
+    assert y.dtype == dtype
+    for name, a, r, e in zip(("y", "dx", "dw", "db"), got, want, err):
+        if a is not None:
+            near(a, r, HALF[dtype] * r.abs() * (1 + 1e-2) + 1.1 * U * e
+                 + 1e-38, f"{name} {tuple(x.shape)} {dtype}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", NORM_SHAPES)
+def test_norm(device, dtype, rows, dim):
+    x = rand(rows, dim, dtype=dtype, device=device, scale=2.0, shift=1.0)
+    check_norm(x, rand(dim, dtype=dtype, device=device, seed=1),
+               rand(dim, dtype=dtype, device=device, seed=2),
+               rand(rows, dim, dtype=dtype, device=device, seed=3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("weight,bias", [(False, False), (True, False),
+                                         (False, True)])
+def test_norm_without_parameters(device, weight, bias):
+    x = rand(2, 5, 96, device=device)
+    check_norm(x, rand(96, device=device, seed=1) if weight else None,
+               rand(96, device=device, seed=2) if bias else None,
+               rand(2, 5, 96, device=device, seed=3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_layouts(device):
+    """Transposed, sliced, misaligned and expanded inputs and gradients."""
+    w, b = rand(64, device=device, seed=1), rand(64, device=device, seed=2)
+    base = rand(64, 40, device=device)
+    dy = rand(40, 64, device=device, seed=3)
+    check_norm(base.t(), w, b, dy)
+    check_norm(rand(40, 130, device=device)[:, 1:129:2], w, b, dy)
+    check_norm(rand(40 * 64 + 1, device=device)[1:].view(40, 64), w, b, dy)
+    check_norm(base.t().contiguous(), w, b,
+               rand(1, 64, device=device).expand(40, 64))
+    check_norm(rand(40, 64, device=device), rand(65, device=device)[1:], b,
+               dy)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_offset(device):
+    """A mean a thousand deviations away costs what its own size costs."""
+    x = rand(20, 256, device=device, shift=1000.0)
+    check_norm(x, rand(256, device=device, seed=1),
+               rand(256, device=device, seed=2),
+               rand(20, 256, device=device, seed=3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_constant_rows_and_non_finite(device):
+    x = torch.full((4, 128), 3.0, device=device)
+    y = ops.layer_norm(x)
+    assert torch.equal(y, torch.zeros_like(x))
+    x[1, 7] = math.inf
+    x[2, 9] = math.nan
+    y = ops.layer_norm(x)
+    assert y[1].isnan().all() and y[2].isnan().all()
+    assert torch.equal(y[0], torch.zeros_like(y[0]))
+    assert torch.equal(y[3], torch.zeros_like(y[3]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_no_rows(device):
+    x = torch.empty(0, 32, device=device, requires_grad=True)
+    w = torch.ones(32, device=device, requires_grad=True)
+    y = ops.layer_norm(x, w)
+    assert y.shape == (0, 32)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+    assert dx.shape == (0, 32) and torch.equal(dw, torch.zeros_like(dw))
+
+
+def test_norm_refusals():
+    x = torch.randn(3, 8)
+    with pytest.raises(TypeError):
+        ops.layer_norm(x.double())
+    with pytest.raises(TypeError):
+        ops.layer_norm([1.0])
+    with pytest.raises(ValueError):
+        ops.layer_norm(torch.tensor(1.0))
+    with pytest.raises(ValueError):
+        ops.layer_norm(torch.empty(3, 0))
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, torch.ones(7))
+    with pytest.raises(TypeError):
+        ops.layer_norm(x, torch.ones(8, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, torch.ones(8), torch.ones(1, 8))
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, eps=-1.0)
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, eps=math.nan)
+
+
+# -------------------------------------------------------------------- loss
+
+LOSS_SHAPES = [(1, 1, 1), (7, 256, 1000), (33, 65, 129), (100, 300, 515),
+               (128, 128, 128), (129, 31, 2000), (300, 64, 127),
+               (2, 513, 300)]
+
+
+def check_loss(x, w, y, b, ignore=-100, reduction="mean", scale=1.0,
+               want_grads=True):
+    dtype = x.dtype
+    x2, y1 = x.reshape(-1, x.shape[-1]), y.reshape(-1)
+    rows, lse, z = loss64(x2.cpu(), w.cpu(), y1.cpu(),
+                          None if b is None else b.cpu(), ignore)
+    # a logit's error, and through it the loss's (exp and log add a few U)
+    za = x2.cpu().double().abs() @ w.cpu().double().abs().t()
+    if b is not None:
+        za = za + b.cpu().double().abs().nan_to_num(posinf=0.0)
+    ez = (x.shape[-1] + 8) * U * za.max(-1).values
+    er = 2 * ez + U * (lse.abs() + w.shape[0] + 16) + U * rows.abs()
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)
+              if t is not None]
+    bl = leaves[2] if b is not None else None
+    out = ops.linear_cross_entropy(leaves[0], leaves[1], y, bl,
+                                   ignore_index=ignore, reduction=reduction)
+    assert out.dtype == torch.float32
+    keep = y1.cpu() != ignore
+    count = keep.sum().double()
+    er = torch.where(keep, er, torch.zeros_like(er))
+    if reduction == "none":
+        near(out, rows.view(y.shape), er.view(y.shape), "rows")
+        up = rand(*y.shape, device=x.device, seed=9) if y.dim() else \
+            torch.ones_like(out)
+        row_grad = up.reshape(-1).double().cpu()
+    else:
+        total = rows.sum() / (count if reduction == "mean" else 1)
+        bound = er.sum() / (count if reduction == "mean" else 1)
+        near(out, total, bound + 2 * U * total.abs(), reduction)
+        up = torch.tensor(scale, device=x.device)
+        row_grad = torch.full((len(y1),), float(scale), dtype=torch.float64)
+        if reduction == "mean":
+            row_grad = row_grad / count
+    if not want_grads:
+        return out, None
+    grads = torch.autograd.grad(out, leaves, up)
+    dx, dw, db, p = loss_grads64(x2.cpu(), w.cpu(), y1.cpu(),
+                                 None if b is None else b.cpu(), ignore,
+                                 row_grad)
+    # p: relative error 2 ez (exponent) + its exponent's own rounding, and for
+    # bf16 one rounding of p itself
+    spread = (z - lse[:, None]).abs().nan_to_num(posinf=0.0)
+    soft = torch.exp(z - lse[:, None]) * row_grad.abs()[:, None]
+    ep = soft * (2 * ez[:, None] + U * (2 * spread + w.shape[0] + 24))
+    ep = ep + p.abs() * 4 * U
+    # the exponential instruction gives 0 below the smallest normal, 2^-126,
+    # and so do the low parts of a split p: at most 2^-126 lost to each,
+    # which x or w of any size multiplies
+    ep = ep + 2.0 ** -124
+    if dtype == torch.bfloat16:
+        ep = ep + p.abs() * HALF[dtype] * 1.01
+    ep = torch.where(keep[:, None], ep, torch.zeros_like(ep))
+    xa, wa = x2.cpu().double().abs(), w.cpu().double().abs()
+    n, v = p.shape
+    ex = ep @ wa + (v + 8) * U * (p.abs() @ wa)
+    ew = ep.t() @ xa + (n + 8) * U * (p.abs().t() @ xa)
+    eb = ep.sum(0) + (n + 8) * U * p.abs().sum(0)
+    got = [grads[0].reshape(-1, x.shape[-1]), grads[1]]
+    want, err = [dx, dw], [ex, ew]
+    if b is not None:
+        got.append(grads[2]); want.append(db); err.append(eb)
+    for name, a, r, e in zip(("dx", "dw", "db"), got, want, err):
+        near(a, r, HALF[dtype] * r.abs() * 1.02 + e + 1e-38,
+             f"{name} {tuple(x.shape)} {w.shape[0]} {dtype}")
+    return out, grads
+
+
+def loss_inputs(rows, dim, vocab, dtype, device, bias=True):
+    x = rand(rows, dim, dtype=dtype, device=device)
+    w = rand(vocab, dim, dtype=dtype, device=device, seed=1,
+             scale=2 / math.sqrt(dim))
+    b = rand(vocab, dtype=dtype, device=device, seed=2) if bias else None
+    g = torch.Generator().manual_seed(rows + vocab)
+    y = torch.randint(0, vocab, (rows,), generator=g)
+    y[0] = vocab - 1
+    if rows > 3:
+        y[2] = -100
+        y[3] = 0
+    return x, w, y.to(device), b
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,vocab", LOSS_SHAPES)
+def test_loss(device, dtype, rows, dim, vocab):
+    x, w, y, b = loss_inputs(rows, dim, vocab, dtype, device)
+    check_loss(x, w, y, b)
+    check_loss(x, w, y, None, reduction="sum", scale=-0.5)
+    check_loss(x.view(1, rows, dim), w, y.view(1, rows), b, reduction="none")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_single_row_without_leading_axis(device):
+    x, w, y, b = loss_inputs(1, 40, 77, torch.float32, device)
+    check_loss(x[0], w, y[0], b, reduction="none")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_loss_in_pieces(dtype):
+    """More logits than one piece of the vocabulary holds."""
+    rows, vocab = 2100, 33000 if dtype == torch.float32 else 64100
+    assert rows * vocab * (4 if dtype == torch.float32 else 2) > 256 << 20
+    x, w, y, b = loss_inputs(rows, 24, vocab, dtype, "cuda")
+    check_loss(x, w, y, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_every_row_ignored(device):
+    x, w, y, b = loss_inputs(5, 16, 30, torch.float32, device)
+    y = torch.full_like(y, -100)
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    mean = ops.linear_cross_entropy(x, w, y, b)
+    assert mean.isnan()
+    for g in torch.autograd.grad(mean, (x, w, b)):
+        assert torch.equal(g, torch.zeros_like(g))
+    total = ops.linear_cross_entropy(x, w, y, b, reduction="sum")
+    assert total == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_no_rows(device):
+    x = torch.empty(0, 8, device=device, requires_grad=True)
+    w = torch.randn(5, 8, device=device, requires_grad=True)
+    y = torch.empty(0, dtype=torch.int64, device=device)
+    assert ops.linear_cross_entropy(x, w, y).isnan()
+    total = ops.linear_cross_entropy(x, w, y, reduction="sum")
+    assert total == 0
+    dx, dw = torch.autograd.grad(total, (x, w))
+    assert dx.shape == x.shape and torch.equal(dw, torch.zeros_like(dw))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_switched_off_words(device):
+    x, w, y, b = loss_inputs(20, 32, 300, torch.float32, device)
+    b[5:290] = -math.inf
+    y = torch.where(y == -100, y, y % 5)
+    check_loss(x, w, y, b)
+    out = ops.linear_cross_entropy(x, w, torch.full_like(y, 7), b,
+                                   reduction="none")
+    assert torch.isposinf(out).all()         # a switched-off word as target
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_large_logits(device):
+    """Logits of hundreds: the running maximum keeps the sums finite."""
+    x, w, y, b = loss_inputs(16, 64, 400, torch.float32, device)
+    check_loss(x * 100, w, y, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [-1, 50, 1 << 40])
+def test_loss_target_outside_the_vocabulary(device, bad):
+    x, w, y, b = loss_inputs(6, 16, 50, torch.float32, device)
+    y[4] = bad
+    x.requires_grad_()
+    rows = ops.linear_cross_entropy(x, w, y, b, reduction="none")
+    assert rows[4].isnan() and not rows[[0, 1, 2, 3, 5]].isnan().any()
+    dx, = torch.autograd.grad(rows.sum(), x)
+    assert dx[4].isnan().all()
+    assert not dx[[0, 1, 2, 3, 5]].isnan().any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_ignore_index_in_the_vocabulary(device):
+    x, w, y, b = loss_inputs(12, 16, 50, torch.float32, device)
+    y[1] = 3
+    y[y == -100] = 3
+    check_loss(x, w, y, b, ignore=3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_layouts(device):
+    x, w, y, b = loss_inputs(40, 64, 90, torch.float32, device)
+    check_loss(x.t().contiguous().t(), w, y, b)
+    check_loss(x[:, ::2], w[:, 1::2], y, b)
+    wide = torch.zeros(90 * 64 + 1, device=device)
+    wide[1:] = w.reshape(-1)
+    check_loss(x, wide[1:].view(90, 64), y[::2].repeat_interleave(2), b)
+
+
+def test_loss_refusals():
+    x, w, y, b = loss_inputs(4, 8, 10, torch.float32, "cpu")
+    f = ops.linear_cross_entropy
+    with pytest.raises(TypeError):
+        f(x.half(), w.half(), y)
+    with pytest.raises(TypeError):
+        f(x, w.bfloat16(), y)
+    with pytest.raises(TypeError):
+        f(x, w, y.int())
+    with pytest.raises(ValueError):
+        f(x, w[:, :7], y)
+    with pytest.raises(ValueError):
+        f(x, w[0], y)
+    with pytest.raises(ValueError):
+        f(x, w[:0], y)
+    with pytest.raises(ValueError):
+        f(x, w, y[:3])
+    with pytest.raises(ValueError):
+        f(x, w, y, b[:9])
+    with pytest.raises(ValueError):
+        f(x, w, y, reduction="max")
+
+
+# ----------------------------------------------------- 8-bit activations
+
+ACT_SHAPES = [(1, 1), (3, 7), (5, 127), (9, 128), (4, 129), (16, 300),
+              (7, 1000), (33, 1024)]
+
+
+def check_gelu(x, dy):
+    dtype = x.dtype
+    leaf = x.detach().clone().requires_grad_()
+    y = ops.gelu_act8(leaf)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    want = gelu64(x)
+    # Phi: 1.2e-5 of the tail in bf16 kernels, 5e-7 in fp32, and the
+    # exponent's rounding; all against |x| Phi <= |x|
+    k = 2e-5 if dtype == torch.bfloat16 else 1e-6
+    near(y, want, HALF[dtype] * want.abs() * 1.01
+         + k * want.abs() + 4 * U * x.double().abs() + 1e-38, "y")
+    v = stored64(x)
+    slope = gelu_slope64(v)
+    d = dy.double()
+    near(dx, d * slope, HALF[dtype] * (d * slope).abs() * 1.01
+         + d.abs() * (k + 8 * U) * (1 + v.abs()) + 1e-38, "dx")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", ACT_SHAPES)
+def test_gelu(device, dtype, rows, dim):
+    check_gelu(rand(rows, dim, dtype=dtype, device=device, scale=2.0),
+               rand(rows, dim, dtype=dtype, device=device, seed=1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gelu_scales(device):
+    """Exponents at their borders: 127 * 2^e and one step beyond, subnormal,
+    tiny, huge and all-zero blocks."""
+    tops = [127.0, 127.00001, 126.99999, 254.0, 1.984375, 1.9843751, 1.0,
+            2.0 ** -120, 2.0 ** -126, 1e-40, 3.0e38, 0.0, 128.0, 64.0, 63.5]
+    x = rand(len(tops), 128, device=device)
+    x = x.clamp(-1, 1) * torch.tensor(tops, device=device)[:, None]
+    x[:, 3] = torch.tensor(tops, device=device)
+    x[:, 5] = -torch.tensor(tops, device=device)
+    check_gelu(x, torch.ones_like(x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gelu_far_values(device):
+    x = torch.linspace(-40, 40, 1000, device=device)[None]
+    check_gelu(x, torch.ones_like(x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_gelu_non_finite_block(device, bad):
+    x = rand(2, 300, device=device)
+    x[0, 140] = bad
+    x.requires_grad_()
+    y = ops.gelu_act8(x)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert dx[0, 128:256].isnan().all()
+    assert not dx[0, :128].isnan().any() and not dx[0, 256:].isnan().any()
+    assert not dx[1].isnan().any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_act8_layouts_and_empty(device):
+    x = rand(256, 40, device=device).t()
+    check_gelu(x, rand(40, 256, device=device, seed=1))
+    flat = rand(40 * 128 + 1, device=device)[1:].view(40, 128)
+    check_gelu(flat, rand(1, 128, device=device).expand(40, 128))
+    e = torch.empty(0, 64, device=device, requires_grad=True)
+    y = ops.gelu_act8(e)
+    assert torch.autograd.grad(y, e, torch.empty_like(y))[0].shape == e.shape
+
+
+LINEAR_SHAPES = [(1, 1, 1), (7, 33, 5), (64, 128, 128), (130, 300, 129),
+                 (300, 257, 64), (1000, 40, 200), (2, 512, 1000)]
+
+
+def check_linear(x, w, b, dy):
+    dtype = x.dtype
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)
+              if t is not None]
+    y = ops.linear_act8(leaves[0], leaves[1],
+                        leaves[2] if b is not None else None)
+    grads = torch.autograd.grad(y, leaves, dy)
+    n, m = w.shape[1], w.shape[0]
+    x2, dy2 = x.reshape(-1, n).double(), dy.reshape(-1, m).double()
+    wd = w.double()
+    bd = 0 if b is None else b.double()
+    k = len(x2)
+    s = stored64(x.reshape(-1, n))
+    want = [(x2 @ wd.t() + bd).view(y.shape), (dy2 @ wd).view(x.shape),
+            dy2.t() @ s, dy2.sum(0)]
+    mags = [(x2.abs() @ wd.abs().t()
+             + (bd.abs() if b is not None else 0)).view(y.shape),
+            (dy2.abs() @ wd.abs()).view(x.shape), dy2.abs().t() @ s.abs(),
+            dy2.abs().sum(0)]
+    for name, a, r, e, c in zip(("y", "dx", "dw", "db"), (y, *grads), want,
+                                mags, (n, m, k, k)):
+        near(a, r, HALF[dtype] * r.abs() * 1.01 + (c + 8) * U * e + 1e-38,
+             f"{name} {tuple(x.shape)} {m} {dtype}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n,m", LINEAR_SHAPES)
+def test_linear(device, dtype, rows, n, m):
+    check_linear(rand(rows, n, dtype=dtype, device=device),
+                 rand(m, n, dtype=dtype, device=device, seed=1),
+                 rand(m, dtype=dtype, device=device, seed=2),
+                 rand(rows, m, dtype=dtype, device=device, seed=3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_layouts(device):
+    x = rand(3, 11, 64, device=device)
+    w, b = rand(30, 64, device=device, seed=1), rand(30, device=device)
+    dy = rand(3, 11, 30, device=device, seed=2)
+    check_linear(x, w, None, dy)
+    check_linear(x.transpose(0, 1).contiguous().transpose(0, 1), w, b, dy)
+    check_linear(x, rand(64, 30, device=device).t(), b,
+                 rand(1, 1, 30, device=device).expand(3, 11, 30))
+    check_linear(rand(11, 130, device=device)[:, 1:129:2], w, b,
+                 rand(30, 11, device=device).t())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_wide_range(device):
+    """fp32 values of very different size: the product keeps fp32's bits."""
+    x = rand(50, 96, device=device) * torch.exp2(
+        torch.arange(96, device=device) % 40 - 20.0)
+    check_linear(x, rand(20, 96, device=device, seed=1), None,
+                 rand(50, 20, device=device, seed=2, scale=1e-6))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_no_rows(device):
+    x = torch.empty(0, 8, device=device, requires_grad=True)
+    w = torch.randn(4, 8, device=device, requires_grad=True)
+    b = torch.randn(4, device=device, requires_grad=True)
+    y = ops.linear_act8(x, w, b)
+    assert y.shape == (0, 4)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert dx.shape == (0, 8)
+    assert torch.equal(dw, torch.zeros_like(dw))
+    assert torch.equal(db, torch.zeros_like(db))
+
+
+def test_act8_refusals():
+    x = torch.randn(3, 8)
+    with pytest.raises(TypeError):
+        ops.gelu_act8(x.double())
+    with pytest.raises(ValueError):
+        ops.gelu_act8(torch.tensor(1.0))
+    with pytest.raises(ValueError):
+        ops.linear_act8(x, torch.randn(8))
+    with pytest.raises(ValueError):
+        ops.linear_act8(x, torch.randn(4, 7))
+    with pytest.raises(ValueError):
+        ops.linear_act8(x, torch.randn(4, 8), torch.randn(3))
+    with pytest.raises(TypeError):
+        ops.linear_act8(x, torch.randn(4, 8).bfloat16())
+
+
+# --------------------------------------------- populations (torch.func)
+
+def loss_fn(w, b, x, y):
+    return ops.linear_cross_entropy(x, w, y, b)
+
+
+def norm_fn(w, b, x, y):
+    return ops.layer_norm(x, w, b)
+
+
+def gelu_linear_fn(w, b, x, y):
+    return ops.gelu_act8(ops.linear_act8(x, w, b))
+
+
+def population(fn, clients, device, dtype=torch.float32, seed=0):
+    n, d, v = 9, 40, 23
+    x = rand(clients, n, d, device=device, dtype=dtype, seed=seed)
+    y = torch.randint(0, v, (clients, n),
+                      generator=torch.Generator().manual_seed(1)).to(device)
+    y[0, 1] = -100
+    m = d if fn is norm_fn else v
+    shape = (d,) if fn is norm_fn else (v, d)
+    w = rand(clients, *shape, device=device, dtype=dtype, seed=seed + 1)
+    b = rand(clients, m, device=device, dtype=dtype, seed=seed + 2)
+    up = {loss_fn: rand(clients, device=device, seed=3),
+          norm_fn: rand(clients, n, d, device=device, dtype=dtype, seed=3),
+          gelu_linear_fn: rand(clients, n, v, device=device, dtype=dtype,
+                               seed=3)}[fn]
+    return w, b, x, y, up
+
+
+def one_by_one(fn, w, b, x, y, up):
+    """Each client alone through ordinary autograd."""
+    outs = []
+    for i in range(len(x)):
+        leaves = [t.detach().clone().requires_grad_()
+                  for t in (w[i], b[i], x[i])]
+        out = fn(*leaves, y[i])
+        outs.append((out.detach(), *torch.autograd.grad(out, leaves, up[i])))
+    return [torch.stack(t) for t in zip(*outs)]
+
+
+FNS = [loss_fn, norm_fn, gelu_linear_fn]
+
+
+def close(a, b, dtype=torch.float32):
+    """Two runs of the same sums in another order or kernel."""
+    tol = 1e-5 if dtype == torch.float32 else 2.0 ** -6
+    assert a.shape == b.shape
+    scale = b.double().abs().max().item() + 1e-30
+    assert (a.double() - b.double()).abs().max().item() <= tol * scale
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fn", FNS)
+@pytest.mark.parametrize("shared", [True, False])
+def test_vmap_of_vjp(device, dtype, fn, shared):
+    w, b, x, y, up = population(fn, 4, device, dtype)
+    if shared:
+        w, b = w[:1].expand_as(w), b[:1].expand_as(b)
+    want = one_by_one(fn, w, b, x, y, up)
+
+    def step(w, b, x, y, up):
+        out, pull = torch.func.vjp(lambda *a: fn(*a, y), w, b, x)
+        return (out, *pull(up))
+    if shared:
+        got = torch.func.vmap(step, in_dims=(None, None, 0, 0, 0))(
+            w[0], b[0], x, y, up)
+    else:
+        got = torch.func.vmap(step)(w, b, x, y, up)
+    for g, r in zip(got, want):
+        close(g, r, dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+@pytest.mark.parametrize("shared", [True, False])
+def test_grad_of_vmap(device, fn, shared):
+    w, b, x, y, up = population(fn, 4, device)
+    if shared:
+        w, b = w[:1].expand_as(w), b[:1].expand_as(b)
+    want = one_by_one(fn, w, b, x, y, up)
+    dims = (None, None, 0, 0) if shared else (0, 0, 0, 0)
+
+    def total(w, b, x):
+        return (torch.func.vmap(fn, in_dims=dims)(w, b, x, y) * up).sum()
+    args = (w[0], b[0], x) if shared else (w, b, x)
+    got = torch.func.grad(total, argnums=(0, 1, 2))(*args)
+    for i, (g, r) in enumerate(zip(got, want[1:])):
+        close(g, r.sum(0) if shared and i < 2 else r)
+    # and by ordinary autograd through the vmap
+    leaves = [t.detach().clone().requires_grad_() for t in args]
+    for g, r in zip(torch.autograd.grad(total(*leaves), leaves), got):
+        close(g, r)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_vmap_other_axes(device, fn):
+    """Client axes that are not the first, and inputs without one."""
+    w, b, x, y, up = population(fn, 4, device)
+    want = torch.stack([fn(w[i], b[i], x[i], y[i]) for i in range(4)])
+    got = torch.func.vmap(fn, in_dims=(-1, 1, 1, 1))(
+        w.movedim(0, -1), b.movedim(0, 1), x.movedim(0, 1), y.movedim(0, 1))
+    close(got, want)
+    got = torch.func.vmap(fn, in_dims=(0, None, None, None))(
+        w, b[0], x[0], y[0])
+    close(got, torch.stack([fn(w[i], b[0], x[0], y[0]) for i in range(4)]))
+    # no input of the operator depends on the client
+    got = torch.func.vmap(lambda s: fn(w[0], b[0], x[0], y[0]) * s)(
+        torch.arange(4.0, device=device))
+    close(got[1], fn(w[0], b[0], x[0], y[0]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_vmap_chunks(device, fn):
+    w, b, x, y, up = population(fn, 5, device)
+    whole = torch.func.vmap(fn, in_dims=(None, None, 0, 0))(w[0], b[0], x, y)
+    parts = torch.func.vmap(fn, in_dims=(None, None, 0, 0), chunk_size=2)(
+        w[0], b[0], x, y)
+    close(parts, whole)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_vmap_loss_rows(device):
+    w, b, x, y, _ = population(loss_fn, 3, device)
+    f = lambda x, y: ops.linear_cross_entropy(x, w[0], y, b[0],
+                                              reduction="none")
+    got = torch.func.vmap(f)(x, y)
+    close(got, torch.stack([f(x[i], y[i]) for i in range(3)]))
+    g = torch.func.vmap(torch.func.grad(lambda x, y: f(x, y).square().sum()))
+    want = []
+    for i in range(3):
+        leaf = x[i].clone().requires_grad_()
+        want.append(torch.autograd.grad(f(leaf, y[i]).square().sum(),
+                                        leaf)[0])
+    close(g(x, y), torch.stack(want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_nested_vmap_refused(device, fn):
+    w, b, x, y, _ = population(fn, 4, device)
+    inner = torch.func.vmap(fn)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.vmap(inner)(w.unflatten(0, (2, 2)), b.unflatten(0, (2, 2)),
+                               x.unflatten(0, (2, 2)), y.unflatten(0, (2, 2)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_second_gradient_refused(device, fn):
+    w, b, x, y, up = population(fn, 1, device)
+    leaves = [t[0].clone().requires_grad_() for t in (w, b, x)]
+    out = (fn(*leaves, y[0]) ** 2).sum()
+    first = torch.autograd.grad(out, leaves, create_graph=True)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.autograd.grad(sum(g.square().sum() for g in first), leaves)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_partial_gradients(device, fn):
+    """Any subset of the inputs, and no gradient at all."""
+    w, b, x, y, up = population(fn, 1, device)
+    want = one_by_one(fn, w, b, x, y, up)
+    for i in range(3):
+        leaves = [w[0].clone(), b[0].clone(), x[0].clone()]
+        leaves[i].requires_grad_()
+        out = fn(*leaves, y[0])
+        close(torch.autograd.grad(out, leaves[i], up[0])[0], want[1 + i][0])
+    with torch.no_grad():
+        close(fn(w[0], b[0], x[0], y[0]), want[0][0])
+
+
+def test_gradients_against_differences():
+    """The 64-bit definitions' central differences along a direction."""
+    x, w, y, b = loss_inputs(9, 24, 50, torch.float32, "cpu")
+    vx, vw = rand(9, 24, seed=5).double(), rand(50, 24, seed=6).double()
+    h = 1e-5
+
+    def mean64(t):
+        r = loss64(x.double() + t * vx, w.double() + t * vw, y, b, -100)[0]
+        return r.sum() / (y != -100).sum()
+    slope = (mean64(h) - mean64(-h)) / (2 * h)
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+    gx, gw = torch.autograd.grad(ops.linear_cross_entropy(*leaves, y, b),
+                                 leaves)
+    got = (gx.double() * vx).sum() + (gw.double() * vw).sum()
+    assert abs(got - slope) <= 1e-5 * (1 + abs(slope))
+
+    dy = rand(9, 24, seed=7)
+    g = rand(24, seed=8)
+
+    def norm_at(t):
+        z = x.double() + t * vx
+        c = z - z.mean(-1, keepdim=True)
+        return (dy.double() * c / (c.square().mean(-1, keepdim=True)
+                                   + 1e-5).sqrt() * g.double()).sum()
+    slope = (norm_at(h) - norm_at(-h)) / (2 * h)
+    leaf = x.clone().requires_grad_()
+    gx, = torch.autograd.grad(ops.layer_norm(leaf, g), leaf, dy)
+    assert abs((gx.double() * vx).sum() - slope) <= 1e-4 * (1 + abs(slope))
+
+
+# --------------------------------------------------- streams and graphs
+
+@gpu
+@pytest.mark.parametrize("fn", FNS)
+def test_results_repeat(fn):
+    w, b, x, y, up = population(fn, 6, "cuda")
+    first = one_by_one(fn, w, b, x, y, up)
+    for _ in range(3):
+        for a, r in zip(one_by_one(fn, w, b, x, y, up), first):
+            assert torch.equal(a, r)
+
+
+@gpu
+@pytest.mark.parametrize("fn", FNS)
+def test_side_stream(fn):
+    w, b, x, y, up = population(fn, 2, "cuda")
+    want = one_by_one(fn, w, b, x, y, up)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = one_by_one(fn, w, b, x, y, up)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, r in zip(got, want):
+        assert torch.equal(a, r)
+
+
+@gpu
+@pytest.mark.parametrize("fn", FNS)
+@pytest.mark.parametrize("rows", [9, 600])
+def test_captured_population_step(fn, rows):
+    """A vmapped step in two captured graphs, replayed in turn on new
+    inputs, with eager work between the replays."""
+    def step(w, b, x, y, up):
+        out, pull = torch.func.vjp(lambda *a: fn(*a, y), w, b, x)
+        return (out, *pull(up))
+    run = torch.func.vmap(step)
+    w, b, x, y, up = population(fn, 3, "cuda")
+    reps = -(-rows // 9)
+    x, y = x.repeat(1, reps, 1)[:, :rows], y.repeat(1, reps)[:, :rows]
+    if fn is not loss_fn:
+        up = up.repeat(1, reps, 1)[:, :rows]
+    static = [t.contiguous().clone() for t in (w, b, x, y, up)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            run(*static)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(*static))
+        graphs.append(g)
+    for i in range(4):
+        for t in static:
+            if t.is_floating_point():
+                t.copy_(torch.randn(t.shape, device="cuda"))
+        graphs[i % 2].replay()
+        want = run(*static)
+        torch.cuda.synchronize()
+        for a, r in zip(outs[i % 2], want):
+            assert torch.equal(a, r)
