@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <limits>
 #include <optional>
 #include <tuple>
@@ -247,7 +248,11 @@ Tensor gelu_backward_t(const Tensor& dy, const Tensor& q, const Tensor& e) {
 
 // ---------------------------------------------------------------- products
 
-void check_tiles(long long m, long long n) {
+// ld: the longest row of an operand
+void check_tiles(long long m, long long n, long long k, long long ld) {
+  // offsets within a tile of 256 rows are 32 bits
+  TORCH_CHECK(std::max({m, n, k}) < (1ll << 31) - 4096 && ld < 1ll << 22,
+              "product of ", m, " x ", n, " x ", k, " is too large");
   TORCH_CHECK(ceil_div(m, 128) * ceil_div(n, 128) < (1ll << 24),
               "product of ", m, " x ", n, " is too large for one launch");
 }
@@ -263,7 +268,7 @@ Mat mat(const Tensor& t, long long group) {
 // out = A B (+ bias) with the contraction cut where the output alone would
 // not fill the chip
 void run_gemm(Gemm& g, const Tensor& like) {
-  const int splits = gemm_splits(g.groups, g.m, g.n, g.k);
+  const int splits = gemm_splits(g);
   const hipStream_t s = stream_of(like);
   if (splits == 1) {
     gemm(g, s);
@@ -287,7 +292,7 @@ Tensor linear_forward_t(const Tensor& x, const Tensor& w, const OptTensor& b) {
   const long long wg = group_stride(w, groups, 2, "weight");
   const long long out = w.size(-2);
   TORCH_CHECK(w.size(-1) == in, "weight does not match x");
-  check_tiles(rows, out);
+  check_tiles(rows, out, in, in);
   c10::DeviceGuard guard(x.device());
   Tensor y = at::empty({groups, rows, out}, x.options());
   if (y.numel() == 0) return y;
@@ -322,7 +327,7 @@ Tensor linear_grad_input_t(const Tensor& dy, const Tensor& w) {
   const long long wg = group_stride(w, groups, 2, "weight");
   const long long in = w.size(-1);
   TORCH_CHECK(w.size(-2) == out, "weight does not match dy");
-  check_tiles(rows, in);
+  check_tiles(rows, in, out, std::max(in, out));
   c10::DeviceGuard guard(dy.device());
   Tensor dx = at::empty({groups, rows, in}, dy.options());
   if (dx.numel() == 0) return dx;
@@ -352,7 +357,7 @@ Tensor linear_grad_weight_t(const Tensor& dy, const Tensor& q,
   const long long groups = dy.size(0), rows = dy.size(1), out = dy.size(2),
                   in = q.size(2);
   check_groups(groups);
-  check_tiles(out, in);
+  check_tiles(out, in, rows, std::max(in, out));
   c10::DeviceGuard guard(dy.device());
   if (rows == 0 || out == 0)
     return at::zeros({groups, out, in}, dy.options());
@@ -406,7 +411,7 @@ Loss loss_args(const Tensor& x, const Tensor& w, const Tensor& target,
     l.bias = bias->data_ptr();
     l.bias_group = group_stride(*bias, l.groups, 1, "bias");
   }
-  check_tiles(l.vocab, l.rows);
+  check_tiles(l.vocab, l.rows, l.dim, l.dim);
   return l;
 }
 
@@ -427,7 +432,10 @@ std::tuple<Tensor, Tensor, Tensor> loss_forward_t(
         reduction == 2 ? std::numeric_limits<double>::quiet_NaN() : 0.0;
     return {at::full({l.groups}, empty, count.options()), lse, count};
   }
-  Tensor part = floats(x, {l.groups, loss_tiles(l.vocab), l.rows, 2});
+  int tile_m, tile_n;
+  loss_tile(l, &tile_m, &tile_n);
+  Tensor part =
+      floats(x, {l.groups, ceil_div(l.vocab, tile_m), l.rows, 2});
   Tensor picked = at::empty_like(lse);
   Tensor loss, sums;
   if (reduction != 0) {
@@ -476,44 +484,58 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
   // 256 MiB hold it in the last-level cache between the kernel that writes
   // it and the two products that read it.
   const long long size = x.element_size();
-  const long long ld = ceil_div(l.rows, 128) * 128;
-  long long piece = (256ll << 20) / (l.groups * ld * size) / 128 * 128;
+  int tile, tile_n;
+  loss_tile(l, &tile, &tile_n);
+  const long long ld = ceil_div(l.rows, tile_n) * tile_n;
+  check_tiles(l.vocab, l.rows, l.dim, ld);
+  long long piece = (256ll << 20) / (l.groups * ld * size) / tile * tile;
   piece = std::max<long long>(piece, 512);
-  piece = std::min(piece, ceil_div(l.vocab, 128) * 128);
+  piece = std::min(piece, ceil_div(l.vocab, tile) * tile);
   // pieces of nearly equal size
   const long long pieces = ceil_div(l.vocab, piece);
-  piece = ceil_div(ceil_div(l.vocab, pieces), 128) * 128;
+  piece = ceil_div(ceil_div(l.vocab, pieces), tile) * tile;
   Tensor pt = at::empty({l.groups, piece, ld}, x.options());
 
-  const int splits = gemm_splits(l.groups, l.rows, l.dim,
-                                 std::min(piece, l.vocab));
+  Gemm gx = {};
+  gx.a_kmajor = gx.b_kmajor = true;
+  gx.ta = gx.tb = gx.tout = l.t;
+  gx.groups = l.groups;
+  gx.m = l.rows;
+  gx.n = l.dim;
+  gx.k = std::min(piece, l.vocab);
+  gx.out = dx.data_ptr();
+  gx.out_ld = l.dim;
+  gx.out_group = l.rows * l.dim;
+  const int splits = gemm_splits(gx);
   Tensor xsum;
   const bool parts = splits > 1 || l.vocab > piece;
   if (want_x && parts) xsum = floats(x, {splits, l.groups, l.rows, l.dim});
 
+  Scale scale = {grad.data_ptr<float>(),
+                 reduction == 2 ? count.data_ptr<float>() : nullptr};
+  Tensor top, ratio;
+  if (reduction == 0) {
+    top = floats(x, {l.groups});
+    ratio = floats(x, {l.groups, l.rows});
+    row_scale(grad.data_ptr<float>(), l.groups, l.rows,
+              top.data_ptr<float>(), ratio.data_ptr<float>(), s);
+    scale.num = top.data_ptr<float>();
+  }
+
   for (long long v0 = 0; v0 < l.vocab; v0 += piece) {
     const long long nv = std::min(piece, l.vocab - v0);
-    loss_logit_grad(l, v0, nv, lse.data_ptr<float>(), grad.data_ptr<float>(),
-                    reduction ? 1 : l.rows, reduction ? 0 : 1,
-                    reduction == 2 ? count.data_ptr<float>() : nullptr,
+    loss_logit_grad(l, v0, nv, lse.data_ptr<float>(),
+                    reduction ? nullptr : ratio.data_ptr<float>(),
                     pt.data_ptr(), ld, piece * ld, s);
     Mat pm = mat(pt, piece * ld);
     pm.padded = true;
     if (want_x) {
-      Gemm g = {};
+      Gemm g = gx;
       g.a = pm;
-      g.a_kmajor = true;
       g.b = l.w;
       g.b.p = static_cast<const char*>(l.w.p) + v0 * l.dim * size;
-      g.b_kmajor = true;
-      g.ta = g.tb = g.tout = l.t;
-      g.groups = l.groups;
-      g.m = l.rows;
-      g.n = l.dim;
       g.k = nv;
-      g.out = dx.data_ptr();
-      g.out_ld = l.dim;
-      g.out_group = l.rows * l.dim;
+      g.scale = scale;
       if (parts) {
         g.partial = xsum.data_ptr<float>();
         g.splits = splits;
@@ -534,11 +556,13 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
       g.out = static_cast<char*>(dw.data_ptr()) + v0 * l.dim * size;
       g.out_ld = l.dim;
       g.out_group = l.vocab * l.dim;
+      g.scale = scale;
       run_gemm(g, x);
     }
     if (want_b)
       rowsum(pt.data_ptr(), ld, piece * ld, l.groups, nv, ld,
-             static_cast<char*>(db.data_ptr()) + v0 * size, l.vocab, l.t, s);
+             static_cast<char*>(db.data_ptr()) + v0 * size, l.vocab, scale, l.t,
+             s);
   }
   if (want_x && parts)
     join_partials(xsum.data_ptr<float>(), splits, l.groups, l.rows, l.dim,

@@ -25,12 +25,12 @@
 #include "token_device.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace token_ops {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 128;
+constexpr int kThreads = 256;          // of the small kernels below
 
 enum Src { F32, BF16, ACT8 };
 enum Epi { STORE, LSE, GRAD };
@@ -40,19 +40,28 @@ template <> struct SrcOf<F32> { using T = float; static constexpr int P = 3; };
 template <> struct SrcOf<BF16> { using T = bf16; static constexpr int P = 1; };
 template <> struct SrcOf<ACT8> { using T = int8_t; static constexpr int P = 1; };
 
+// Waves of a block along m and n, and each wave's 32 x 32 tiles.
+template <int WM_, int WN_, int MF_, int NF_, int BK_> struct Shape {
+  static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, BK = BK_;
+  static constexpr int BM = WM * MF * 32, BN = WN * NF * 32;
+  static constexpr int THREADS = WM * WN * 64;
+};
+using Small = Shape<2, 2, 2, 2, 64>;       // 128 x 128, 4 waves
+using Large = Shape<2, 4, 4, 2, 64>;       // 256 x 256, 8 waves
+
 // What a kernel knows of an operand: `rows` of the output it feeds (m or n),
 // and how far the contiguous axis may be read.
 struct Op {
   const void* p;
   long long ld, group;
-  long long rows, ext;
+  int rows, ext;
   const uint8_t* e;
   long long e_ld, e_group;
 };
 
 struct Params {
   Op a, b;
-  long long k;
+  int k;
   int tiles_m, tiles_n, splits;
   // STORE
   void* out;
@@ -67,10 +76,16 @@ struct Params {
   float2* part;
   float* picked;
   const float* lse;
-  const float* grad;
-  long long grad_g, grad_n;
-  const float* count;
+  const float* ratio;     // [groups][n], null: all ones
+  Scale scale;            // of what STORE writes
 };
+
+__device__ __forceinline__ float scale_of(const Scale& s, long long g) {
+  if (!s.num) return 1.f;
+  if (!s.den) return s.num[g];
+  // nothing counted: nothing to scale
+  return s.den[g] == 0.f ? 0.f : s.num[g] / s.den[g];
+}
 
 // Three bf16 parts of 8 floats, packed in pairs.
 __device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&o)[3]) {
@@ -91,133 +106,194 @@ __device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&o)[3]) {
   }
 }
 
+// Wide accesses at an element's alignment: rows of any length and stride are
+// read 16 bytes at a time.
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+typedef u32x2 u32x2_u __attribute__((aligned(1)));
+
 template <Src S> struct Raw { u32x4 v; };
-template <> struct Raw<F32> { float v[8]; };
+template <> struct Raw<F32> { f32x4 x, y; };
 template <> struct Raw<ACT8> { u32x2 v; uint32_t e; };
 
-// Moves one operand's 128 x BK tile: global -> registers -> LDS.
-template <Src S, bool KM, bool VEC, int BK>
+// Moves one operand's ROWS x BK tile: global -> registers -> LDS, in chunks
+// of 8 values along the contiguous axis.
+template <Src S, bool KM, int ROWS, int THREADS, int BK, int SETS_>
 struct Loader {
   using T = typename SrcOf<S>::T;
   static constexpr int P = SrcOf<S>::P;
-  static constexpr int N = kTile * BK / 8 / kThreads;   // chunks a thread
-  static constexpr int PLANE = kTile * BK;              // bf16 values
-  const T* p;
-  const uint8_t* e;
+  static constexpr int N = ROWS * BK / 8 / THREADS;     // chunks a thread
+  static constexpr int PLANE = ROWS * BK;               // bf16 values
+  static_assert(N >= 1 && N * 8 * THREADS == ROWS * BK);
+  const char* base;      // the next step's tile, the same for all threads
+  const uint8_t* ebase;
+  uint32_t off[N], eoff[N];                // bytes from there to a chunk
   long long ld, e_ld;
-  long long ext;       // end of the contiguous axis
-  long long row0;      // first row of the tile ([m][k]) or column ([k][m])
-  long long rows;
-  long long kend;
-  Raw<S> raw[N];
+  int ext, left[N];      // [k][m]: end of a row, values from a chunk to it
+  int kend, krows;       // end of this block's and of the whole contraction
+  static constexpr int SETS = SETS_;      // steps on their way
+  Raw<S> raws[SETS][N];
 
-  __device__ __forceinline__ void init(const Op& o, long long g,
-                                       long long tile, long long kend_) {
-    p = static_cast<const T*>(o.p) + g * o.group;
-    e = o.e ? o.e + g * o.e_group : nullptr;
+  __device__ __forceinline__ void init(const Op& o, long long g, int tile,
+                                       int k0, int kend_, int krows_) {
     ld = o.ld;
     e_ld = o.e_ld;
     ext = o.ext;
-    rows = o.rows;
-    row0 = tile * kTile;
     kend = kend_;
-  }
-
-  // r, c: row and first column in memory; lim: columns beyond are zero
-  __device__ __forceinline__ void fetch(Raw<S>& w, bool ok, long long r,
-                                        long long c, long long lim) {
-    const T* q = p + r * ld + c;
-    if constexpr (S == F32) {
-      if constexpr (VEC) {
-        f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-        if (ok && c < lim) x = *reinterpret_cast<const f32x4*>(q);
-        if (ok && c + 4 < lim) y = *reinterpret_cast<const f32x4*>(q + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { w.v[j] = x[j]; w.v[4 + j] = y[j]; }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          w.v[j] = (ok && c + j < lim) ? q[j] : 0.f;
-      }
-    } else if constexpr (S == BF16) {
-      w.v = u32x4{0, 0, 0, 0};
-      if constexpr (VEC) {
-        if (ok && c < lim) w.v = *reinterpret_cast<const u32x4*>(q);
-      } else {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (ok && c + j < lim)
-            w.v[j >> 1] |= (uint32_t)h[j] << (16 * (j & 1));
-      }
-    } else {
-      w.v = u32x2{0, 0};
-      w.e = 0;
-      if (ok && c < lim) w.e = e[r * e_ld + (c >> 7)];
-      if constexpr (VEC) {
-        if (ok && c < lim) w.v = *reinterpret_cast<const u32x2*>(q);
-      } else {
-        const uint8_t* h = reinterpret_cast<const uint8_t*>(q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (ok && c + j < lim)
-            w.v[j >> 2] |= (uint32_t)h[j] << (8 * (j & 3));
-      }
-    }
-  }
-
-  __device__ __forceinline__ void load(long long k0) {
+    krows = krows_;
+    const int row0 = tile * ROWS;
+    base = static_cast<const char*>(o.p)
+        + (g * o.group + (KM ? k0 * ld + row0 : row0 * ld + k0)) * sizeof(T);
+    if constexpr (S == ACT8)
+      ebase = o.e + g * o.e_group + k0 * e_ld + (row0 >> 7);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int id = i * kThreads + threadIdx.x;
+      const int id = i * THREADS + threadIdx.x;
+      // Rows (or columns) beyond the operand feed outputs that nobody
+      // stores: read its last ones for them.
       if constexpr (KM) {
-        const long long k = k0 + (id >> 4);
-        fetch(raw[i], k < kend, k, row0 + (id & 15) * 8, ext);
+        const int k = id / (ROWS / 8);
+        int c = id % (ROWS / 8) * 8;
+        const int last = ((ext - 1) & ~7) - row0;
+        if (c > last) c = last;
+        left[i] = ext - row0 - c;
+        off[i] = (uint32_t)((k * ld + c) * sizeof(T));
+        if constexpr (S == ACT8)
+          eoff[i] = (uint32_t)(k * e_ld + (c >> 7));
       } else {
-        const long long r = row0 + id / (BK / 8);
-        const long long lim = kend < ext ? kend : ext;
-        fetch(raw[i], r < rows, r, k0 + (id % (BK / 8)) * 8, lim);
+        int r = id / (BK / 8);
+        if (r >= o.rows - row0) r = o.rows - row0 - 1;
+        off[i] = (uint32_t)((r * ld + id % (BK / 8) * 8) * sizeof(T));
       }
     }
   }
 
-  __device__ __forceinline__ void store(bf16* lds) const {
+  __device__ __forceinline__ const T* at(int i) const {
+    return reinterpret_cast<const T*>(base + off[i]);
+  }
+  __device__ __forceinline__ void advance() {
+    base += (KM ? BK * ld : (long long)BK) * (long long)sizeof(T);
+    if constexpr (S == ACT8) ebase += BK * e_ld;
+  }
+
+  // Whether the step from k0 can be read as it lies.  A [k][m] row's last
+  // chunk may run up to 7 values into the rows behind it, which have to be
+  // there.
+  __device__ __forceinline__ bool whole(int k0) const {
+    return k0 + BK <= kend
+        && (!KM || (ext & 7) == 0 || (krows - k0 - BK) * ld >= 8);
+  }
+
+  template <int SET> __device__ __forceinline__ void load_whole() {
+    Raw<S>(&raw)[N] = raws[SET];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int id = i * kThreads + threadIdx.x;
+      if constexpr (S == F32) {
+        raw[i].x = *reinterpret_cast<const f32x4_u*>(at(i));
+        raw[i].y = *reinterpret_cast<const f32x4_u*>(at(i) + 4);
+      } else if constexpr (S == BF16) {
+        raw[i].v = *reinterpret_cast<const u32x4_u*>(at(i));
+      } else {
+        raw[i].v = *reinterpret_cast<const u32x2_u*>(at(i));
+        raw[i].e = ebase[eoff[i]];
+      }
+    }
+    advance();
+  }
+
+  template <int SET> __device__ __forceinline__ void load(int k0) {
+    if (whole(k0)) load_whole<SET>(); else tail(k0, raws[SET]);
+  }
+
+  // The last step: each value is checked, and zero beyond the contraction.
+  __device__ __forceinline__ void tail(int k0, Raw<S> (&raw)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = i * THREADS + threadIdx.x;
+      int valid;
+      if constexpr (KM) {
+        const bool in = k0 + id / (ROWS / 8) < kend;
+        valid = !in ? 0 : left[i] < 8 ? left[i] : 8;
+      } else {
+        valid = kend - (k0 + id % (BK / 8) * 8);
+      }
+      if constexpr (S == F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          raw[i].x[j] = j < valid ? at(i)[j] : 0.f;
+          raw[i].y[j] = 4 + j < valid ? at(i)[4 + j] : 0.f;
+        }
+      } else if constexpr (S == BF16) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(at(i));
+        raw[i].v = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < valid) raw[i].v[j >> 1] |= (uint32_t)h[j] << (16 * (j & 1));
+      } else {
+        const uint8_t* h = reinterpret_cast<const uint8_t*>(at(i));
+        raw[i].v = u32x2{0, 0};
+        raw[i].e = valid > 0 ? ebase[eoff[i]] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < valid) raw[i].v[j >> 2] |= (uint32_t)h[j] << (8 * (j & 3));
+      }
+    }
+    advance();
+  }
+
+  template <int SET>
+  __device__ __forceinline__ void store(bf16* lds) const {
+    const Raw<S>(&raw)[N] = raws[SET];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = i * THREADS + threadIdx.x;
       int at;
       if constexpr (KM) {
-        const int k = id >> 4, c = id & 15;
-        at = k * kTile + (((c >> 1) ^ (2 * (k & 3))) << 4) + (c & 1) * 8;
+        const int k = id / (ROWS / 8), c = id % (ROWS / 8);
+        at = k * ROWS + (((c >> 1) ^ (2 * (k & 3))) << 4) + (c & 1) * 8;
       } else {
-        constexpr int CH = BK / 8;
-        const int r = id / CH, c = id % CH;
-        const int sw = CH == 8 ? (r & 7) : ((r >> 1) & 3);
-        at = r * BK + ((c ^ sw) << 3);
+        const int r = id / (BK / 8), c = id % (BK / 8);
+        at = r * BK + ((c ^ swizzle(r)) << 3);
       }
       u32x4 o[3];
       if constexpr (S == F32) {
-        split3(raw[i].v, o);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = raw[i].x[j];
+          v[4 + j] = raw[i].y[j];
+        }
+        split3(v, o);
       } else if constexpr (S == BF16) {
         o[0] = raw[i].v;
       } else {
+        // (q + 128) * unit - 128 * unit, exact: bytes convert unsigned
         const float unit = __uint_as_float(raw[i].e << 23);
+        const float off = -128.f * unit;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v[2];
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = raw[i].v[h] ^ 0x80808080u;
+          float v[4];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int b = 2 * j + t;
-            v[t] = (float)(int8_t)(raw[i].v[b >> 2] >> (8 * (b & 3))) * unit;
-          }
-          o[0][j] = __builtin_amdgcn_perm(__float_as_uint(v[1]),
-                                          __float_as_uint(v[0]), 0x07060302u);
+          for (int t = 0; t < 4; ++t)
+            v[t] = fmaf((float)((w >> (8 * t)) & 0xffu), unit, off);
+          o[0][2 * h] = __builtin_amdgcn_perm(
+              __float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
+          o[0][2 * h + 1] = __builtin_amdgcn_perm(
+              __float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u);
         }
       }
 #pragma unroll
       for (int q = 0; q < P; ++q)
         *reinterpret_cast<u32x4*>(lds + q * PLANE + at) = o[q];
     }
+  }
+
+  // 16-byte columns of an [m][BK] row are swapped about by the row so that 16
+  // neighbouring rows' reads of one column touch each of the 64 banks once.
+  static __device__ __forceinline__ int swizzle(int r) {
+    constexpr int C = BK / 8;                 // columns; 16 / C rows a bank row
+    return r / (16 / C) % C;
   }
 
   // Fragment of the 32 rows from `base`, contraction step ks of 16.
@@ -230,20 +306,19 @@ struct Loader {
       const int c = (base >> 4) + ((lane >> 4) & 1);
       const int k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
       // k and k + 4 have the same low bits, so the same swizzle
-      const bf16* q = lds + k * kTile + ((c ^ (2 * (k & 3))) << 4)
+      const bf16* q = lds + k * ROWS + ((c ^ (2 * (k & 3))) << 4)
           + (i & 3) * 4;
       union { s4 h[2]; bf16x8 v; } u;
       typedef __attribute__((address_space(3))) s4* lds_s4;
       u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(q));
       u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s4)(q + 4 * kTile));
+          (lds_s4)(q + 4 * ROWS));
       return u.v;
     } else {
-      constexpr int CH = BK / 8;
       const int r = base + (lane & 31);
       const int c = ks * 2 + (lane >> 5);
-      const int sw = CH == 8 ? (r & 7) : ((r >> 1) & 3);
-      return *reinterpret_cast<const bf16x8*>(lds + r * BK + ((c ^ sw) << 3));
+      return *reinterpret_cast<const bf16x8*>(
+          lds + r * BK + ((c ^ swizzle(r)) << 3));
     }
   }
 };
@@ -255,15 +330,24 @@ __device__ __forceinline__ int acc_row(int r, int lane) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <Src SA, bool KMA, Src SB, bool KMB, bool VEC, Epi E>
-__global__ __launch_bounds__(kThreads)
+template <Src S>
+__device__ __forceinline__ float bias_at(const void* p, long long i) {
+  return S == F32 ? static_cast<const float*>(p)[i]
+                  : (float)static_cast<const bf16*>(p)[i];
+}
+
+template <Src SA, bool KMA, Src SB, bool KMB, typename H, Epi E>
+__global__ __launch_bounds__(H::THREADS)
 void gemm_kernel(Params p) {
   constexpr int PA = SrcOf<SA>::P, PB = SrcOf<SB>::P;
-  constexpr int BK = (PA == 3 || PB == 3) ? 32 : 64;
-  using LA = Loader<SA, KMA, VEC, BK>;
-  using LB = Loader<SB, KMB, VEC, BK>;
-  __shared__ __attribute__((aligned(16))) bf16 sa[PA * LA::PLANE];
-  __shared__ __attribute__((aligned(16))) bf16 sb[PB * LB::PLANE];
+  constexpr int MF = H::MF, NF = H::NF;
+  constexpr int BK = (PA == 3 || PB == 3) ? 16 : H::BK;
+  // a step of fp32 is short against memory's latency: two are on their way
+  constexpr int SETS = BK == 16 ? 2 : 1;
+  using LA = Loader<SA, KMA, H::BM, H::THREADS, BK, SETS>;
+  using LB = Loader<SB, KMB, H::BN, H::THREADS, BK, SETS>;
+  __shared__ __attribute__((aligned(16))) bf16 sa[2][PA * LA::PLANE];
+  __shared__ __attribute__((aligned(16))) bf16 sb[2][PB * LB::PLANE];
 
   // Blocks go round robin over the 8 XCDs; give each a contiguous run of
   // tiles, ordered in bands of 8 so that neighbours share operands in its L2.
@@ -280,93 +364,183 @@ void gemm_kernel(Params p) {
   }
   const int split = blockIdx.y;
   const long long g = blockIdx.z;
-  const long long steps = (p.k + BK - 1) / BK;
-  const long long s0 = steps * split / p.splits;
-  const long long s1 = steps * (split + 1) / p.splits;
-  const long long kend = s1 * BK < p.k ? s1 * BK : p.k;
+  const int steps = (p.k + BK - 1) / BK;
+  const int s0 = (int)((long long)steps * split / p.splits);
+  const int s1 = (int)((long long)steps * (split + 1) / p.splits);
+  const int kend = (long long)s1 * BK < p.k ? s1 * BK : p.k;
 
   LA la;
   LB lb;
-  la.init(p.a, g, tm, kend);
-  lb.init(p.b, g, tn, kend);
+  la.init(p.a, g, tm, s0 * BK, kend, p.k);
+  lb.init(p.b, g, tn, s0 * BK, kend, p.k);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int wm = wave / H::WN * (MF * 32), wn = wave % H::WN * (NF * 32);
 
-  f32x16 acc[2][2];
+  f32x16 acc[MF][NF];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < MF; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NF; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  if (s0 < s1) {
-    la.load(s0 * BK);
-    lb.load(s0 * BK);
-  }
-  for (long long s = s0; s < s1; ++s) {
+  // Units of a step: one 16-deep slice of one row of the wave's tiles.
+  constexpr int UNITS = BK / 16 * MF;
+  bf16x8 fb[NF][PB];
+  auto read_b = [&](const bf16* tb, int ks) {
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int q = 0; q < PB; ++q)
+        fb[j][q] = LB::frag(tb + q * LB::PLANE, wn + j * 32, ks);
+  };
+  auto read_a = [&](const bf16* ta, int u, bf16x8 (&fa)[PA]) {
+#pragma unroll
+    for (int q = 0; q < PA; ++q)
+      fa[q] = LA::frag(ta + q * LA::PLANE, wm + u % MF * 32, u / MF);
+  };
+  auto products = [&](int i, const bf16x8 (&fa)[PA]) {
+#pragma unroll
+    for (int qa = 0; qa < PA; ++qa)
+#pragma unroll
+      for (int qb = 0; qb < PB; ++qb) {
+        if (qa + qb > 2) continue;
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              fa[qa], fb[j][qb], acc[i][j], 0, 0, 0);
+      }
+  };
+  auto multiply = [&](const bf16* ta, const bf16* tb, auto from) {
+#pragma unroll
+    for (int u = from(); u < UNITS; ++u) {
+      if (u % MF == 0) read_b(tb, u / MF);
+      bf16x8 fa[PA];
+      read_a(ta, u, fa);
+      products(u % MF, fa);
+    }
+  };
+  constexpr int FIRST = MF;      // units that cover conversion and writing
+  using First = std::integral_constant<int, FIRST>;
+  using None = std::integral_constant<int, 0>;
+
+  // Two tiles in LDS: one is multiplied while the next is converted and
+  // written, and the one or two after it are on their way in registers.  One
+  // barrier a step: behind it the tile to multiply is whole and the other
+  // one free.
+  auto fast_step = [&](auto cur, auto set) {
     __syncthreads();
-    la.store(sa);
-    lb.store(sb);
+    // The fragments come first: a read cannot pass the writes below.
+    __builtin_amdgcn_sched_barrier(0);
+    read_b(sb[cur()], 0);
+    bf16x8 fa[FIRST][PA];
+#pragma unroll
+    for (int u = 0; u < FIRST; ++u) read_a(sa[cur()], u, fa[u]);
+    __builtin_amdgcn_sched_barrier(0);
+    la.template store<decltype(set)::value>(sa[cur() ^ 1]);
+    lb.template store<decltype(set)::value>(sb[cur() ^ 1]);
+#pragma unroll
+    for (int u = 0; u < FIRST; ++u) products(u, fa[u]);
+    // one product, then what the vector unit does in its shadow: its work
+    // spread over the products (8-bit values need the most conversion)
+    constexpr int SHADE = PA == 1 && SB == ACT8 ? 12 : 4;
+#pragma unroll
+    for (int q = 0; q < FIRST * NF * (PA * PB > 3 ? 6 : PA * PB); ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, SHADE, 0);
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+    }
+    // Left to itself the compiler moves these loads behind the products.
+    __builtin_amdgcn_sched_barrier(0);
+    la.template load_whole<decltype(set)::value>();
+    lb.template load_whole<decltype(set)::value>();
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(sa[cur()], sb[cur()], First());
+  };
+  auto checked_step = [&](int s, auto cur, auto set) {
     __syncthreads();
     if (s + 1 < s1) {
-      la.load((s + 1) * BK);
-      lb.load((s + 1) * BK);
+      la.template store<decltype(set)::value>(sa[cur() ^ 1]);
+      lb.template store<decltype(set)::value>(sb[cur() ^ 1]);
     }
-#pragma unroll
-    for (int ks = 0; ks < BK / 16; ++ks) {
-      bf16x8 fa[2][PA], fb[2][PB];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int q = 0; q < PA; ++q)
-          fa[i][q] = LA::frag(sa + q * LA::PLANE, wm + i * 32, ks);
-#pragma unroll
-        for (int q = 0; q < PB; ++q)
-          fb[i][q] = LB::frag(sb + q * LB::PLANE, wn + i * 32, ks);
-      }
-#pragma unroll
-      for (int qa = 0; qa < PA; ++qa)
-#pragma unroll
-        for (int qb = 0; qb < PB; ++qb) {
-          if (qa + qb > 2) continue;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  fa[i][qa], fb[j][qb], acc[i][j], 0, 0, 0);
-        }
+    if (s + 1 + SETS < s1) {
+      la.template load<decltype(set)::value>((s + 1 + SETS) * BK);
+      lb.template load<decltype(set)::value>((s + 1 + SETS) * BK);
+    }
+    multiply(sa[cur()], sb[cur()], None());
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  // the register set of odd steps
+  using Odd = std::integral_constant<int, SETS - 1>;
+
+  int s = s0;
+  // Every step before the last is whole unless an operand's rows are shorter
+  // than a chunk; without a branch, conversion and loads go between the
+  // matrix instructions.
+  if (s0 + SETS + 3 < s1 && (!KMA || p.a.ld >= 8) && (!KMB || p.b.ld >= 8)) {
+    la.template load_whole<0>();
+    lb.template load_whole<0>();
+    la.template store<0>(sa[0]);
+    lb.template store<0>(sb[0]);
+    la.template load_whole<Odd::value>();
+    lb.template load_whole<Odd::value>();
+    if (SETS == 2) {
+      la.template load_whole<0>();
+      lb.template load_whole<0>();
+    }
+    do {
+      fast_step(Zero(), Odd());
+      fast_step(One(), Zero());
+      s += 2;
+    } while (s + SETS + 3 < s1);
+  } else {
+    if (s0 < s1) {
+      la.template load<0>(s0 * BK);
+      lb.template load<0>(s0 * BK);
+      la.template store<0>(sa[0]);
+      lb.template store<0>(sb[0]);
+    }
+    if (s0 + 1 < s1) {
+      la.template load<Odd::value>((s0 + 1) * BK);
+      lb.template load<Odd::value>((s0 + 1) * BK);
+    }
+    if (SETS == 2 && s0 + 2 < s1) {
+      la.template load<0>((s0 + 2) * BK);
+      lb.template load<0>((s0 + 2) * BK);
     }
   }
+  for (; s < s1; s += 2) {
+    checked_step(s, Zero(), Odd());
+    if (s + 1 < s1) checked_step(s + 1, One(), Zero());
+  }
 
-  const long long m0 = (long long)tm * kTile + wm;
-  const long long n0 = (long long)tn * kTile + wn;
-  const long long M = p.a.rows, N = p.b.rows;
+  const int m0 = tm * H::BM + wm, n0 = tn * H::BN + wn;
+  const int M = p.a.rows, N = p.b.rows;
 
   if constexpr (E == STORE) {
+    const float scale = scale_of(p.scale, g);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long long n = n0 + j * 32 + (lane & 31);
+    for (int j = 0; j < NF; ++j) {
+      const int n = n0 + j * 32 + (lane & 31);
       if (n >= N) continue;
       float bias = 0.f;
       if (p.bias && !p.partial)
-        bias = p.out_f32
-            ? static_cast<const float*>(p.bias)[g * p.bias_group + n]
-            : (float)static_cast<const bf16*>(p.bias)[g * p.bias_group + n];
+        bias = p.out_f32 ? bias_at<F32>(p.bias, g * p.bias_group + n)
+                         : bias_at<BF16>(p.bias, g * p.bias_group + n);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < MF; ++i) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const long long m = m0 + i * 32 + acc_row(r, lane);
+          const int m = m0 + i * 32 + acc_row(r, lane);
           if (m >= M) continue;
-          const float v = acc[i][j][r] + bias;
+          const float v = fmaf(acc[i][j][r], scale, bias);
           if (p.partial) {
             float* o = p.partial
                 + (((long long)split * gridDim.z + g) * M + m) * N + n;
             *o = p.accumulate ? *o + v : v;
           } else {
-            const long long at = g * p.out_group + m * p.out_ld + n;
+            const long long at = g * p.out_group + (long long)m * p.out_ld + n;
             if (p.out_f32)
               static_cast<float*>(p.out)[at] = v;
             else
@@ -377,101 +551,117 @@ void gemm_kernel(Params p) {
     }
   }
 
+  if constexpr (E != STORE) {
+    // the tile's biases, -inf beyond the vocabulary
+    float* sbias = reinterpret_cast<float*>(sa[0]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < H::BM; i += H::THREADS) {
+      const int v = tm * H::BM + i;
+      sbias[i] = v >= M ? -INFINITY
+          : p.bias ? bias_at<SA>(p.bias, g * p.bias_group + v) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(
+            sbias + wm + i * 32 + acc_row(4 * q, lane));
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // a row beyond the vocabulary holds another's product: replace
+            const int m = m0 + i * 32 + acc_row(4 * q + r, lane);
+            acc[i][j][4 * q + r] =
+                m < M ? acc[i][j][4 * q + r] + b[r] : b[r];
+          }
+      }
+  }
+
   if constexpr (E == LSE) {
     // Tokens lie along lanes, the vocabulary along registers: a token's
     // maximum and sum need one exchange between the lane halves and one
-    // between the two waves that share its column.
-    __shared__ float2 half[2][kTile];
-    float bias[2][16];
+    // between the waves that share its column.
+    float2* half = reinterpret_cast<float2*>(sb[0]);     // [WM][BN]
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const long long v = m0 + i * 32 + acc_row(r, lane);
-        float b = 0.f;
-        if (p.bias && v < M)
-          b = SA == F32
-              ? static_cast<const float*>(p.bias)[g * p.bias_group + v]
-              : (float)static_cast<const bf16*>(p.bias)[g * p.bias_group + v];
-        bias[i][r] = b;
-      }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long long n = n0 + j * 32 + (lane & 31);
+    for (int j = 0; j < NF; ++j) {
+      const int n = n0 + j * 32 + (lane & 31);
       const long long tgt = n < N ? p.target[g * N + n] : -1;
+      // the target's place in this wave's rows, or out of them
+      const long long place = tgt - m0;
+      const int row = place >= 0 && place < MF * 32 && tgt < M ? (int)place
+                                                               : -1;
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const long long v = m0 + i * 32 + acc_row(r, lane);
-          float z = acc[i][j][r] + bias[i][r];
-          if (v >= M) z = -INFINITY;
-          else if (v == tgt) p.picked[g * N + n] = z;
-          acc[i][j][r] = z;
-          mx = fmaxf(mx, z);
+          mx = fmaxf(mx, acc[i][j][r]);
+          if (i * 32 + acc_row(r, lane) == row)
+            p.picked[g * N + n] = acc[i][j][r];
         }
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float ref = mx == -INFINITY ? 0.f : mx;
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           sum += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
       sum += __shfl_xor(sum, 32, 64);
-      if (lane < 32) half[wave >> 1][wn + j * 32 + lane] = make_float2(mx, sum);
+      if (lane < 32)
+        half[wave / H::WN * H::BN + wn + j * 32 + lane] = make_float2(mx, sum);
     }
     __syncthreads();
-    if (threadIdx.x < kTile) {
-      const long long n = (long long)tn * kTile + threadIdx.x;
+    for (int t = threadIdx.x; t < H::BN; t += H::THREADS) {
+      const int n = tn * H::BN + t;
       if (n < N) {
-        const float2 x = half[0][threadIdx.x], y = half[1][threadIdx.x];
-        const float mx = fmaxf(x.x, y.x);
+        float mx = half[t].x;
+#pragma unroll
+        for (int w = 1; w < H::WM; ++w) mx = fmaxf(mx, half[w * H::BN + t].x);
         const float ref = mx == -INFINITY ? 0.f : mx;
-        p.part[(g * p.tiles_m + tm) * N + n] = make_float2(
-            mx, x.y * __builtin_amdgcn_exp2f((x.x - ref) * kLog2e)
-                    + y.y * __builtin_amdgcn_exp2f((y.x - ref) * kLog2e));
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < H::WM; ++w) {
+          const float2 x = half[w * H::BN + t];
+          sum += x.y * __builtin_amdgcn_exp2f((x.x - ref) * kLog2e);
+        }
+        p.part[(g * p.tiles_m + tm) * N + n] = make_float2(mx, sum);
       }
     }
   }
 
   if constexpr (E == GRAD) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long long n = n0 + j * 32 + (lane & 31);
+    for (int j = 0; j < NF; ++j) {
+      const int n = n0 + j * 32 + (lane & 31);
       long long tgt = p.ignore;
-      float lse = 0.f, gr = 0.f;
+      float lse = 0.f, ratio = 1.f;
       if (n < N) {
         tgt = p.target[g * N + n];
         lse = p.lse[g * N + n];
-        gr = p.grad[g * p.grad_g + n * p.grad_n];
-        if (p.count) gr /= p.count[g];
+        if (p.ratio) ratio = p.ratio[g * N + n];
       }
       const bool live = n < N && tgt != p.ignore;
+      const long long place = tgt - p.v0 - m0;
+      const int row = place >= 0 && place < MF * 32 ? (int)place : -1;
+      // whole tiles are written: readers need no bounds
+      const long long at = g * p.out_group
+          + (long long)(m0 + 4 * (lane >> 5)) * p.out_ld + n;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const long long v = m0 + i * 32 + acc_row(r, lane);
-          float d = 0.f;
-          if (live && v < M) {
-            float z = acc[i][j][r];
-            if (p.bias)
-              z += SA == F32
-                  ? static_cast<const float*>(p.bias)[g * p.bias_group + v]
-                  : (float)static_cast<const bf16*>(
-                        p.bias)[g * p.bias_group + v];
-            d = __builtin_amdgcn_exp2f((z - lse) * kLog2e);
-            if (p.v0 + v == tgt) d -= 1.f;
-            d *= gr;
-          }
-          // whole tiles are written: readers need no bounds
-          const long long at = g * p.out_group + v * p.out_ld + n;
+          const int mr = i * 32 + (r & 3) + 8 * (r >> 2);
+          // beyond the vocabulary the logit is -inf: exp gives 0
+          float d = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e);
+          if (mr + 4 * (lane >> 5) == row) d -= 1.f;
+          d = live && m0 + mr + 4 * (lane >> 5) < M ? d * ratio : 0.f;
           if (SA == F32)
-            static_cast<float*>(p.out)[at] = d;
+            static_cast<float*>(p.out)[at + mr * p.out_ld] = d;
           else
-            static_cast<bf16*>(p.out)[at] = (bf16)d;
+            static_cast<bf16*>(p.out)[at + mr * p.out_ld] = (bf16)d;
         }
     }
   }
@@ -584,12 +774,34 @@ void loss_sum_kernel(const double2* __restrict__ sums, long long blocks,
   }
 }
 
+// The largest magnitude of a group's upstream row gradients, and the rows'
+// ratios to it.
+__global__ __launch_bounds__(kThreads)
+void row_scale_kernel(const float* __restrict__ grad, long long rows,
+                      float* __restrict__ top, float* __restrict__ ratio) {
+  __shared__ uint32_t red[4];
+  const long long g = blockIdx.x;
+  uint32_t m = 0;                      // bit patterns order NaN above all
+  for (long long i = threadIdx.x; i < rows; i += kThreads)
+    m = max(m, __float_as_uint(grad[g * rows + i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float t = __uint_as_float(m);
+  if (threadIdx.x == 0) top[g] = t;
+  for (long long i = threadIdx.x; i < rows; i += kThreads)
+    ratio[g * rows + i] = m == 0 ? 0.f : grad[g * rows + i] / t;
+}
+
 // A wave sums a row of the logits' gradient.
 template <typename T>
 __global__ __launch_bounds__(kThreads)
 void rowsum_kernel(const T* __restrict__ pt, long long ld, long long group,
                    long long rows, long long cols, T* out,
-                   long long out_group) {
+                   long long out_group, Scale scale) {
   constexpr int V = Vec16<T>::n;
   const int lane = threadIdx.x & 63;
   const long long g = blockIdx.y;
@@ -604,20 +816,8 @@ void rowsum_kernel(const T* __restrict__ pt, long long ld, long long group,
       for (int j = 0; j < V; ++j) s += v[j];
     }
     s = lanes_sum<64>(s);
-    if (lane == 0) out[g * out_group + r] = from_f<T>(s);
+    if (lane == 0) out[g * out_group + r] = from_f<T>(s * scale_of(scale, g));
   }
-}
-
-bool aligned(const void* p, long long n) {
-  return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0;
-}
-
-// 16-byte loads (8 for 8-bit storage) are possible: aligned rows, and the
-// contiguous axis ends on a whole access.
-bool vector_ok(const Op& o, Src s) {
-  const long long per = s == F32 ? 4 : 8, bytes = s == ACT8 ? 8 : 16;
-  return o.ext % per == 0 && o.ld % per == 0 && o.group % per == 0
-      && aligned(o.p, bytes);
 }
 
 Op make_op(const Mat& m, bool kmajor, long long rows, long long k) {
@@ -625,22 +825,78 @@ Op make_op(const Mat& m, bool kmajor, long long rows, long long k) {
   o.p = m.p;
   o.ld = m.ld;
   o.group = m.group;
-  o.rows = rows;
-  o.ext = m.padded ? m.ld : kmajor ? rows : k;
+  o.rows = (int)rows;
+  o.ext = (int)(m.padded ? m.ld : kmajor ? rows : k);
   o.e = m.e;
   o.e_ld = m.e_ld;
   o.e_group = m.e_group;
   return o;
 }
 
-template <Src SA, bool KMA, Src SB, bool KMB, Epi E>
-void launch(Params& p, long long groups, hipStream_t s) {
+template <Src SA, bool KMA, Src SB, bool KMB, typename H, Epi E>
+void launch_as(Params& p, long long groups, hipStream_t s) {
+  p.tiles_m = (int)ceil_div(p.a.rows, H::BM);
+  p.tiles_n = (int)ceil_div(p.b.rows, H::BN);
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits,
                   (unsigned)groups);
-  if (vector_ok(p.a, SA) && vector_ok(p.b, SB))
-    gemm_kernel<SA, KMA, SB, KMB, true, E><<<grid, kThreads, 0, s>>>(p);
+  gemm_kernel<SA, KMA, SB, KMB, H, E><<<grid, H::THREADS, 0, s>>>(p);
+}
+
+template <Src SA, bool KMA, Src SB, bool KMB, Epi E>
+void launch(Params& p, long long groups, bool large, hipStream_t s) {
+  if (large)
+    launch_as<SA, KMA, SB, KMB, Large, E>(p, groups, s);
   else
-    gemm_kernel<SA, KMA, SB, KMB, false, E><<<grid, kThreads, 0, s>>>(p);
+    launch_as<SA, KMA, SB, KMB, Small, E>(p, groups, s);
+}
+
+// Large or small tiles, and parts of the contraction, by an estimate of the
+// time.  A compute unit works off blocks in rounds, one large or two small at
+// once.  A round's time is its area and its depth plus a fixed part (filling
+// the pipeline, the epilogue), which one large block alone does not hide as
+// well; measured: large tiles are 1.16 times as fast in the long run (bf16
+// 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
+// contractions (fp32 16 x 500 x 5000 x 300: 171 against 197 us) and where
+// few blocks would leave units idle.
+struct Tiling {
+  bool large;
+  int splits;
+};
+
+// `deep`: whether the contraction may be cut into parts, each at least 256
+// deep.  `products`: matrix instructions per multiplication (1, 3 or 6).
+Tiling tiling(long long groups, long long m, long long n, long long k,
+              bool deep, int products) {
+  Tiling best = {false, 1};
+  double least = -1;
+  // 128 x 128 x 1 steps of a compute unit per microsecond
+  const double rate = products == 6 ? 24 : products == 3 ? 45 : 135;
+  const long long most = deep ? std::max<long long>(
+      1, std::min<long long>(k / 256, 64)) : 1;
+  for (int large = 0; large < 2; ++large) {
+    const long long bm = large ? Large::BM : Small::BM;
+    const long long bn = large ? Large::BN : Small::BN;
+    const long long tiles = ceil_div(m, bm) * ceil_div(n, bn) * groups;
+    for (long long splits = 1; splits <= most; ++splits) {
+      const long long blocks = tiles * splits;
+      const double rounds = large
+          ? 4.0 * ceil_div(blocks, 256)
+          : 2.32 * (blocks / 512)
+              + (blocks % 512 == 0 ? 0 : blocks % 512 <= 256 ? 1.4 : 2.32);
+      double us = rounds * (ceil_div(k, splits) + (large ? 92 : 50)) / rate;
+      // the parts are written, read and joined
+      if (splits > 1) us += 4 + (2 * splits + 1) * 4e-6 * m * n * groups / 4;
+      if (least < 0 || us < least) {
+        least = us;
+        best = {large != 0, (int)splits};
+      }
+    }
+  }
+  return best;
+}
+
+int products_of(DType a, bool b_act8) {
+  return a != kF32 ? 1 : b_act8 ? 3 : 6;
 }
 
 unsigned grid_of(long long blocks) {
@@ -650,21 +906,16 @@ unsigned grid_of(long long blocks) {
 
 }  // namespace
 
-// Parts to cut the contraction into: enough blocks for two per compute unit,
-// each part at least 256 deep so that its sum is worth its trip to memory.
-int gemm_splits(long long groups, long long m, long long n, long long k) {
-  const long long tiles = ceil_div(m, kTile) * ceil_div(n, kTile) * groups;
-  const long long want = ceil_div(512, std::max<long long>(tiles, 1));
-  return (int)std::max<long long>(1, std::min(want, k / 256));
+int gemm_splits(const Gemm& g) {
+  return tiling(g.groups, g.m, g.n, g.k, true,
+                products_of(g.ta, g.b.e != nullptr)).splits;
 }
 
 void gemm(const Gemm& g, hipStream_t s) {
   Params p = {};
   p.a = make_op(g.a, g.a_kmajor, g.m, g.k);
   p.b = make_op(g.b, g.b_kmajor, g.n, g.k);
-  p.k = g.k;
-  p.tiles_m = (int)ceil_div(g.m, kTile);
-  p.tiles_n = (int)ceil_div(g.n, kTile);
+  p.k = (int)g.k;
   p.splits = g.partial ? g.splits : 1;
   p.out = g.out;
   p.out_ld = g.out_ld;
@@ -674,19 +925,23 @@ void gemm(const Gemm& g, hipStream_t s) {
   p.bias = g.bias;
   p.bias_group = g.bias_group;
   p.partial = g.partial;
+  p.scale = g.scale;
   const bool f = g.ta == kF32;
+  const bool large = tiling(g.groups, g.m, g.n, g.k, true,
+                            products_of(g.ta, g.b.e != nullptr)).large;
+  const long long n = g.groups;
   if (g.b.e) {                                     // dY' X8
-    if (f) launch<F32, true, ACT8, true, STORE>(p, g.groups, s);
-    else launch<BF16, true, ACT8, true, STORE>(p, g.groups, s);
+    if (f) launch<F32, true, ACT8, true, STORE>(p, n, large, s);
+    else launch<BF16, true, ACT8, true, STORE>(p, n, large, s);
   } else if (!g.a_kmajor && !g.b_kmajor) {         // X W'
-    if (f) launch<F32, false, F32, false, STORE>(p, g.groups, s);
-    else launch<BF16, false, BF16, false, STORE>(p, g.groups, s);
+    if (f) launch<F32, false, F32, false, STORE>(p, n, large, s);
+    else launch<BF16, false, BF16, false, STORE>(p, n, large, s);
   } else if (!g.a_kmajor) {                        // dY W
-    if (f) launch<F32, false, F32, true, STORE>(p, g.groups, s);
-    else launch<BF16, false, BF16, true, STORE>(p, g.groups, s);
+    if (f) launch<F32, false, F32, true, STORE>(p, n, large, s);
+    else launch<BF16, false, BF16, true, STORE>(p, n, large, s);
   } else {                                         // P' W, P stored by word
-    if (f) launch<F32, true, F32, true, STORE>(p, g.groups, s);
-    else launch<BF16, true, BF16, true, STORE>(p, g.groups, s);
+    if (f) launch<F32, true, F32, true, STORE>(p, n, large, s);
+    else launch<BF16, true, BF16, true, STORE>(p, n, large, s);
   }
 }
 
@@ -706,7 +961,12 @@ void join_partials(const float* partial, int splits, long long groups,
         out_group, static_cast<const bf16*>(bias), bias_group);
 }
 
-long long loss_tiles(long long vocab) { return ceil_div(vocab, kTile); }
+void loss_tile(const Loss& l, int* m, int* n) {
+  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
+                            products_of(l.t, false)).large;
+  *m = large ? Large::BM : Small::BM;
+  *n = large ? Large::BN : Small::BN;
+}
 long long loss_sum_blocks(long long rows) { return ceil_div(rows, 32); }
 
 namespace {
@@ -717,9 +977,7 @@ Params loss_params(const Loss& l, long long v0, long long nv) {
   w.p = static_cast<const char*>(w.p) + v0 * w.ld * size;
   p.a = make_op(w, false, nv, l.dim);
   p.b = make_op(l.x, false, l.rows, l.dim);
-  p.k = l.dim;
-  p.tiles_m = (int)ceil_div(nv, kTile);
-  p.tiles_n = (int)ceil_div(l.rows, kTile);
+  p.k = (int)l.dim;
   p.splits = 1;
   p.bias = l.bias ? static_cast<const char*>(l.bias) + v0 * size : nullptr;
   p.bias_group = l.bias_group;
@@ -736,8 +994,10 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
   Params p = loss_params(l, 0, l.vocab);
   p.part = static_cast<float2*>(part);
   p.picked = picked;
-  if (l.t == kF32) launch<F32, false, F32, false, LSE>(p, l.groups, s);
-  else launch<BF16, false, BF16, false, LSE>(p, l.groups, s);
+  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
+                            products_of(l.t, false)).large;
+  if (l.t == kF32) launch<F32, false, F32, false, LSE>(p, l.groups, large, s);
+  else launch<BF16, false, BF16, false, LSE>(p, l.groups, large, s);
   const long long blocks = loss_sum_blocks(l.rows);
   lse_kernel<<<dim3(grid_of(blocks), (unsigned)l.groups), kThreads, 0, s>>>(
       p.part, picked, l.target, l.ignore, l.vocab, p.tiles_m, l.rows, lse,
@@ -748,34 +1008,38 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
 }
 
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
-                     const float* lse, const float* grad, long long grad_g,
-                     long long grad_n, const float* count, void* pt,
+                     const float* lse, const float* ratio, void* pt,
                      long long pt_ld, long long pt_group, hipStream_t s) {
   Params p = loss_params(l, v0, nv);
   p.lse = lse;
-  p.grad = grad;
-  p.grad_g = grad_g;
-  p.grad_n = grad_n;
-  p.count = count;
+  p.ratio = ratio;
   p.out = pt;
   p.out_ld = pt_ld;
   p.out_group = pt_group;
-  if (l.t == kF32) launch<F32, false, F32, false, GRAD>(p, l.groups, s);
-  else launch<BF16, false, BF16, false, GRAD>(p, l.groups, s);
+  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
+                            products_of(l.t, false)).large;
+  if (l.t == kF32) launch<F32, false, F32, false, GRAD>(p, l.groups, large, s);
+  else launch<BF16, false, BF16, false, GRAD>(p, l.groups, large, s);
+}
+
+void row_scale(const float* grad, long long groups, long long rows,
+               float* top, float* ratio, hipStream_t s) {
+  row_scale_kernel<<<dim3((unsigned)groups), kThreads, 0, s>>>(grad, rows,
+                                                               top, ratio);
 }
 
 void rowsum(const void* pt, long long ld, long long group, long long groups,
             long long rows, long long cols, void* out, long long out_group,
-            DType t, hipStream_t s) {
+            const Scale& scale, DType t, hipStream_t s) {
   const dim3 grid(grid_of(ceil_div(rows, 4)), (unsigned)groups);
   if (t == kF32)
     rowsum_kernel<float><<<grid, kThreads, 0, s>>>(
         static_cast<const float*>(pt), ld, group, rows, cols,
-        static_cast<float*>(out), out_group);
+        static_cast<float*>(out), out_group, scale);
   else
     rowsum_kernel<bf16><<<grid, kThreads, 0, s>>>(
         static_cast<const bf16*>(pt), ld, group, rows, cols,
-        static_cast<bf16*>(out), out_group);
+        static_cast<bf16*>(out), out_group, scale);
 }
 
 }  // namespace token_ops

@@ -65,7 +65,14 @@ struct Mat {              // row-major, `ld` elements between rows
   bool padded;            // rows may be read, as zeros, up to `ld`
 };
 
-// out[g][m][n] = sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), 32-bit sums.
+// A factor per group: num[g], or num[g] / den[g] (0 where den is 0), or 1
+// where num is null.
+struct Scale {
+  const float* num;
+  const float* den;
+};
+
+// out[g][m][n] = scale[g] * sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), 32-bit sums.
 //   a_kmajor: A is stored [k][m] instead of [m][k]; likewise b_kmajor.
 // With `partial` set and splits > 1 the contraction is cut into `splits`
 // parts whose sums go to partial[split][g][m][n] and are joined afterwards;
@@ -83,8 +90,10 @@ struct Gemm {
   float* partial;
   int splits;
   bool accumulate;
+  Scale scale;
 };
-int gemm_splits(long long groups, long long m, long long n, long long k);
+// Parts the contraction is best cut into (1: write `out` at once).
+int gemm_splits(const Gemm& g);
 void gemm(const Gemm& g, hipStream_t s);
 // out = sum over splits of partial (+ bias), rounded to tout
 void join_partials(const float* partial, int splits, long long groups,
@@ -102,9 +111,9 @@ struct Loss {
   long long groups, rows, vocab, dim, ignore;
   DType t;
 };
-// number of vocabulary tiles = rows of the (max, sum) partials
-long long loss_tiles(long long vocab);
-// part: [groups][tiles][rows] float2; picked: [groups][rows] float.  Writes
+// Tiles the loss is computed in: m words by n rows.
+void loss_tile(const Loss& l, int* m, int* n);
+// part: [groups][vocabulary tiles][rows] float2; picked: [groups][rows] float.  Writes
 // lse and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
 // group and the number of counted rows, through block_sums
 // [groups][loss_sum_blocks(rows)] double2.
@@ -112,16 +121,19 @@ long long loss_sum_blocks(long long rows);
 void loss_forward(const Loss& l, void* part, float* picked, float* lse,
                   float* row_loss, void* block_sums, float* loss,
                   float* count, bool mean, hipStream_t s);
-// One piece of the vocabulary [v0, v0+nv): pt[g][v][ld] = the loss's
-// gradient in the logits, token-minor, zero beyond rows and nv up to whole
-// tiles.  grad: upstream gradient, one per group or per row.
+// Upstream gradients per row as top[g] * ratio[g][row], |ratio| <= 1.
+void row_scale(const float* grad, long long groups, long long rows,
+               float* top, float* ratio, hipStream_t s);
+// One piece of the vocabulary [v0, v0+nv): pt[g][v][ld] = ratio * (softmax -
+// onehot), token-minor, zero beyond rows and nv up to whole tiles.
+// The group's upstream factor stays out of it: rounded into the bf16 values
+// it would be one relative error, up to 2^-8, common to all of them.
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
-                     const float* lse, const float* grad, long long grad_g,
-                     long long grad_n, const float* count, void* pt,
+                     const float* lse, const float* ratio, void* pt,
                      long long pt_ld, long long pt_group, hipStream_t s);
-// out[g][v] = sum over the row of pt
+// out[g][v] = scale * sum over the row of pt
 void rowsum(const void* pt, long long ld, long long group, long long groups,
             long long rows, long long cols, void* out, long long out_group,
-            DType t, hipStream_t s);
+            const Scale& scale, DType t, hipStream_t s);
 
 }  // namespace token_ops
