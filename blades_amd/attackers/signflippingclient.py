@@ -22,8 +22,7 @@ class SignflippingClient(ByzantineClient):
             data, target = data.to(self.device), target.to(self.device)
             data, target = self.on_train_batch_begin(data=data, target=target)
             self.optimizer.zero_grad()
-            output = self.model(data)
-            loss = torch.clamp(self.loss_func(output, target), 0, 1e5)
+            loss = torch.clamp(self.training_loss(data, target), 0, 1e5)
             loss.backward()
             for _, p in self.model.named_parameters():
                 if p.grad is not None:

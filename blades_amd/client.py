@@ -34,6 +34,7 @@ class BladesClient:
     _is_byzantine: bool = False
     _is_trusted: bool = False
     device: str = "cpu"
+    _head_loss: bool = False
 
     def __init__(self, id: Optional[str] = None, device: Optional[str] = "cpu"):
         self._state = defaultdict(dict)
@@ -95,8 +96,13 @@ class BladesClient:
                 g["lr"] = lr
 
     def set_loss(self, loss_func: str = "crossentropy") -> None:
-        if loss_func == "crossentropy":
+        """``"crossentropy"`` of the model's output, or
+        ``"linear_crossentropy"``: the same value from a model that takes
+        ``targets`` and computes it without the logits
+        (:func:`blades_amd.ops.linear_cross_entropy`)."""
+        if loss_func in ("crossentropy", "linear_crossentropy"):
             self.loss_func = nn.CrossEntropyLoss()
+            self._head_loss = loss_func == "linear_crossentropy"
         else:
             raise NotImplementedError(loss_func)
 
@@ -116,6 +122,12 @@ class BladesClient:
     def on_train_batch_begin(self, data, target, logs=None):
         return data, target
 
+    def training_loss(self, data, target) -> torch.Tensor:
+        """The batch's training loss (see :meth:`set_loss`)."""
+        if self._head_loss:
+            return self.model(data, targets=target)
+        return self.loss_func(self.model(data), target)
+
     def local_training(self, data_batches: list) -> None:
         """Per-batch: zero_grad / forward / clamp(loss) / backward / step
         (reference: client.py:178-193; loss clamp [0, 1e6] at :191)."""
@@ -123,8 +135,7 @@ class BladesClient:
             data, target = data.to(self.device), target.to(self.device)
             data, target = self.on_train_batch_begin(data=data, target=target)
             self.optimizer.zero_grad()
-            output = self.model(data)
-            loss = torch.clamp(self.loss_func(output, target), 0, 1e6)
+            loss = torch.clamp(self.training_loss(data, target), 0, 1e6)
             loss.backward()
             self.optimizer.step()
 

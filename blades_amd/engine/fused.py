@@ -62,10 +62,13 @@ class FusedEngine:
     device : target device
     client_chunk : optional vmap chunk size over the client dim to bound
         activation memory (None = all clients at once)
+    head_loss : train on the loss that ``model(x, targets=y)`` returns, which
+        is computed without the logits
     """
 
     def __init__(self, model: nn.Module, spec: ParamSpec, device,
-                 client_chunk: Optional[int] = None):
+                 client_chunk: Optional[int] = None,
+                 head_loss: bool = False):
         import copy
 
         self.device = torch.device(device)
@@ -75,6 +78,7 @@ class FusedEngine:
         # buffers (none for vmap-safe BN; kept for generality) are shared
         self.buffers = {k: v.detach().clone() for k, v in self.base.named_buffers()}
         self.client_chunk = client_chunk
+        self.head_loss = head_loss
         # NOTE round 2: the direct-MFMA population-conv path (popconv) was
         # REMOVED after losing both of its target configs on hardware —
         # docs/popconv_postmortem.md has the measurements and reasoning.
@@ -83,8 +87,12 @@ class FusedEngine:
     def _loss(self, params_tuple: Tuple[Tensor, ...], x: Tensor, y: Tensor,
               clamp_hi: Tensor, grad_sign: Tensor) -> Tensor:
         params = dict(zip(self.spec.names, params_tuple))
-        out = functional_call(self.base, (params, self.buffers), (x,))
-        loss = self.base_loss(out, y)
+        if self.head_loss:
+            loss = functional_call(self.base, (params, self.buffers), (x,),
+                                   {"targets": y})
+        else:
+            out = functional_call(self.base, (params, self.buffers), (x,))
+            loss = self.base_loss(out, y)
         # reference loss clamp (client.py:191 / signflippingclient.py:17):
         # clamp to [0, hi]; min/minimum keep the same zero-gradient-outside
         # semantics torch.clamp has.  grad_sign folds sign-flip (K13) in:

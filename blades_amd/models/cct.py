@@ -20,6 +20,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .layers import FusedLayerNorm, head_loss, layer_types
+
 
 class DropPath(nn.Module):
     """Stochastic depth per sample."""
@@ -75,19 +77,21 @@ class EncoderLayer(nn.Module):
     """
 
     def __init__(self, dim: int, heads: int, mlp_ratio: float,
-                 dropout: float, attn_dropout: float, drop_path: float):
+                 dropout: float, attn_dropout: float, drop_path: float,
+                 fused_norm: bool = False, act_bits: int = 32):
         super().__init__()
-        self.pre_norm = nn.LayerNorm(dim)
+        norm, linear, self.gelu = layer_types(fused_norm, act_bits)
+        self.pre_norm = norm(dim)
         self.heads = heads
-        self.qkv = nn.Linear(dim, dim * 3, bias=False)
+        self.qkv = linear(dim, dim * 3, bias=False)
         self.attn_dropout = attn_dropout
-        self.proj = nn.Linear(dim, dim)
+        self.proj = linear(dim, dim)
         self.proj_drop = nn.Dropout(dropout)
-        self.norm1 = nn.LayerNorm(dim)
+        self.norm1 = norm(dim)
         hidden = int(dim * mlp_ratio)
-        self.linear1 = nn.Linear(dim, hidden)
+        self.linear1 = linear(dim, hidden)
         self.dropout1 = nn.Dropout(dropout)
-        self.linear2 = nn.Linear(hidden, dim)
+        self.linear2 = linear(hidden, dim)
         self.dropout2 = nn.Dropout(dropout)
         self.drop_path = DropPath(drop_path)
 
@@ -103,7 +107,7 @@ class EncoderLayer(nn.Module):
     def forward(self, x):
         x = x + self.drop_path(self._attn(self.pre_norm(x)))
         x = self.norm1(x)
-        h = self.linear2(self.dropout1(F.gelu(self.linear1(x))))
+        h = self.linear2(self.dropout1(self.gelu(self.linear1(x))))
         return x + self.drop_path(self.dropout2(h))
 
 
@@ -131,7 +135,15 @@ class CCT(nn.Module):
     ``tokenizer='patch'`` + ``pool='seq'`` -> CVT;
     ``tokenizer='patch'`` + ``pool='cls'`` -> ViT-Lite.
     (reference zoo: cctnets/cct.py, cvt.py, vit.py)
+
+    ``fused_norm``: layer norms on :func:`blades_amd.ops.layer_norm`.
+    ``act_bits=8``: the encoder keeps the inputs of its linear layers and
+    GELUs in 8 bits for the backward pass.  Neither changes the parameters.
+    ``forward(x, targets=y)`` returns the mean cross entropy, computed without
+    the logits (``Simulator.run(loss="linear_crossentropy")``).
     """
+
+    supports_head_loss = True
 
     def __init__(self, img_size: int = 32, embedding_dim: int = 128,
                  num_layers: int = 2, num_heads: int = 2, mlp_ratio: float = 1.0,
@@ -140,7 +152,8 @@ class CCT(nn.Module):
                  stochastic_depth: float = 0.1, in_channels: int = 3,
                  positional_embedding: str = "learnable",
                  tokenizer: str = "conv", pool: str = "seq",
-                 patch_size: int = 4):
+                 patch_size: int = 4, fused_norm: bool = False,
+                 act_bits: int = 32):
         super().__init__()
         if tokenizer == "conv":
             self.tokenizer = Tokenizer(n_conv_layers=n_conv_layers,
@@ -170,10 +183,11 @@ class CCT(nn.Module):
         dpr = torch.linspace(0, stochastic_depth, num_layers).tolist()
         self.blocks = nn.ModuleList([
             EncoderLayer(embedding_dim, num_heads, mlp_ratio,
-                         dropout, attn_dropout, dpr[i])
+                         dropout, attn_dropout, dpr[i], fused_norm, act_bits)
             for i in range(num_layers)
         ])
-        self.norm = nn.LayerNorm(embedding_dim)
+        self.norm = (FusedLayerNorm if fused_norm else nn.LayerNorm)(
+            embedding_dim)
         self.attention_pool = nn.Linear(embedding_dim, 1)
         self.fc = nn.Linear(embedding_dim, num_classes)
         self.apply(self._init)
@@ -196,7 +210,8 @@ class CCT(nn.Module):
         pe = torch.where(i.long() % 2 == 0, torch.sin(angle), torch.cos(angle))
         return pe.unsqueeze(0)
 
-    def forward(self, x):
+    def features(self, x):
+        """What the head ``fc`` reads: [B, embedding_dim]."""
         x = self.tokenizer(x)
         if self.pool == "cls":
             cls = self.class_emb.expand(x.shape[0], -1, -1)
@@ -213,7 +228,12 @@ class CCT(nn.Module):
             # sequence pooling: softmax(Wx) over tokens, weighted sum
             w = F.softmax(self.attention_pool(x), dim=1)  # [B, N, 1]
             x = torch.matmul(w.transpose(-1, -2), x).squeeze(-2)
-        return self.fc(x)
+        return x
+
+    def forward(self, x, targets=None):
+        x = self.features(x)
+        return self.fc(x) if targets is None else head_loss(x, self.fc,
+                                                            targets)
 
 
 def cct_2_3x2_32(num_classes: int = 10, img_size: int = 32, **kw) -> CCT:
@@ -238,12 +258,14 @@ def vit_lite_2_4_32(num_classes: int = 10, img_size: int = 32, **kw) -> CCT:
 class CCTNet(nn.Module):
     """Reference-name wrapper (reference: src/blades/models/cifar10/cct.py:7-16)."""
 
+    supports_head_loss = True
+
     def __init__(self, num_classes: int = 10):
         super().__init__()
         self.model = cct_2_3x2_32(num_classes=num_classes)
 
-    def forward(self, x):
-        return self.model(x)
+    def forward(self, x, targets=None):
+        return self.model(x, targets)
 
 
 def create_model():

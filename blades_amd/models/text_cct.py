@@ -21,6 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .cct import DropPath
+from .layers import FusedLayerNorm, head_loss, layer_types
 
 
 class Embedder(nn.Module):
@@ -80,19 +81,21 @@ class MaskedEncoderLayer(nn.Module):
     key-padding mask applied inside SDPA."""
 
     def __init__(self, dim: int, heads: int, mlp_ratio: float,
-                 dropout: float, attn_dropout: float, drop_path: float):
+                 dropout: float, attn_dropout: float, drop_path: float,
+                 fused_norm: bool = False, act_bits: int = 32):
         super().__init__()
-        self.pre_norm = nn.LayerNorm(dim)
+        norm, linear, self.gelu = layer_types(fused_norm, act_bits)
+        self.pre_norm = norm(dim)
         self.heads = heads
-        self.qkv = nn.Linear(dim, dim * 3, bias=False)
+        self.qkv = linear(dim, dim * 3, bias=False)
         self.attn_dropout = attn_dropout
-        self.proj = nn.Linear(dim, dim)
+        self.proj = linear(dim, dim)
         self.proj_drop = nn.Dropout(dropout)
-        self.norm1 = nn.LayerNorm(dim)
+        self.norm1 = norm(dim)
         hidden = int(dim * mlp_ratio)
-        self.linear1 = nn.Linear(dim, hidden)
+        self.linear1 = linear(dim, hidden)
         self.dropout1 = nn.Dropout(dropout)
-        self.linear2 = nn.Linear(hidden, dim)
+        self.linear2 = linear(hidden, dim)
         self.dropout2 = nn.Dropout(dropout)
         self.drop_path = DropPath(drop_path)
 
@@ -112,7 +115,7 @@ class MaskedEncoderLayer(nn.Module):
     def forward(self, x, mask=None):
         x = x + self.drop_path(self._attn(self.pre_norm(x), mask))
         x = self.norm1(x)
-        h = self.linear2(self.dropout1(F.gelu(self.linear1(x))))
+        h = self.linear2(self.dropout1(self.gelu(self.linear1(x))))
         return x + self.drop_path(self.dropout2(h))
 
 
@@ -121,7 +124,8 @@ class MaskedTextClassifier(nn.Module):
 
     def __init__(self, seq_len: int, dim: int, num_layers: int, heads: int,
                  mlp_ratio: float, num_classes: int, dropout: float = 0.0,
-                 attn_dropout: float = 0.1, stochastic_depth: float = 0.1):
+                 attn_dropout: float = 0.1, stochastic_depth: float = 0.1,
+                 fused_norm: bool = False, act_bits: int = 32):
         super().__init__()
         self.pos_emb = nn.Parameter(torch.empty(1, seq_len, dim))
         nn.init.trunc_normal_(self.pos_emb, std=0.2)
@@ -129,13 +133,14 @@ class MaskedTextClassifier(nn.Module):
         dpr = torch.linspace(0, stochastic_depth, num_layers).tolist()
         self.layers = nn.ModuleList([
             MaskedEncoderLayer(dim, heads, mlp_ratio, dropout, attn_dropout,
-                               p)
+                               p, fused_norm, act_bits)
             for p in dpr])
-        self.norm = nn.LayerNorm(dim)
+        self.norm = (FusedLayerNorm if fused_norm else nn.LayerNorm)(dim)
         self.seq_pool = nn.Linear(dim, 1)
         self.fc = nn.Linear(dim, num_classes)
 
-    def forward(self, x, mask=None):
+    def features(self, x, mask=None):
+        """What the head ``fc`` reads: [B, dim]."""
         n = x.shape[1]
         x = self.dropout(x + self.pos_emb[:, :n])
         for layer in self.layers:
@@ -144,11 +149,21 @@ class MaskedTextClassifier(nn.Module):
         w = self.seq_pool(x).squeeze(-1)  # [B, N]
         if mask is not None:
             w = w.masked_fill(~mask[:, :n], float("-inf"))
-        pooled = torch.einsum("bn,bnd->bd", w.softmax(dim=1), x)
-        return self.fc(pooled)
+        return torch.einsum("bn,bnd->bd", w.softmax(dim=1), x)
+
+    def forward(self, x, mask=None, targets=None):
+        pooled = self.features(x, mask)
+        return (self.fc(pooled) if targets is None
+                else head_loss(pooled, self.fc, targets))
 
 
 class TextCCT(nn.Module):
+    """Masked text transformer; ``num_classes`` is the vocabulary for a
+    next-word model.  ``fused_norm``, ``act_bits`` and ``targets`` as for
+    :class:`blades_amd.models.cct.CCT`."""
+
+    supports_head_loss = True
+
     def __init__(self, seq_len: int = 64, word_embedding_dim: int = 300,
                  embedding_dim: int = 128, num_layers: int = 2,
                  num_heads: int = 2, mlp_ratio: float = 1.0,
@@ -167,11 +182,11 @@ class TextCCT(nn.Module):
         self.classifier = MaskedTextClassifier(
             eff_len, dim, num_layers, num_heads, mlp_ratio, num_classes, **kw)
 
-    def forward(self, ids, mask=None):
+    def forward(self, ids, mask=None, targets=None):
         x, mask = self.embedder(ids, mask)
         if self.tokenizer is not None:
             x, mask = self.tokenizer(x, mask)
-        return self.classifier(x, mask)
+        return self.classifier(x, mask, targets)
 
 
 def _cct(layers, heads, ratio, dim, **kw):

@@ -755,7 +755,16 @@ class Simulator:
         client_lr_scheduler=None,
     ) -> List[float]:
         """Run the adversarial training; returns per-round wall-clock seconds
-        (the reference's measurement hook, simulator.py:453-457)."""
+        (the reference's measurement hook, simulator.py:453-457).
+
+        ``loss``: ``"crossentropy"``, or ``"linear_crossentropy"`` for models
+        that compute it from their last linear layer without storing the
+        logits (the transformers; made for large vocabularies)."""
+        head_loss = loss == "linear_crossentropy"
+        if head_loss and not getattr(model, "supports_head_loss", False):
+            raise ValueError(
+                f"loss='linear_crossentropy' needs a model whose forward takes "
+                f"targets; {type(model).__name__} does not")
         reset_model_weights(model)
         model = model.to(self.device)
         self.global_model = model
@@ -782,7 +791,8 @@ class Simulator:
         # engines
         self._loop = LoopEngine(device=self.device)
         self._fused = FusedEngine(model, self._spec, self.device,
-                                  client_chunk=self._client_chunk)
+                                  client_chunk=self._client_chunk,
+                                  head_loss=head_loss)
 
         clients = self.get_clients()
         self.parallel_call(clients, lambda c: c.set_loss(loss))

@@ -38,6 +38,14 @@ def parse_arguments(argv=None):
     parser.add_argument("--num_gpus", type=int, default=4)
     parser.add_argument("--model", type=str, default="cct",
                         help="mlp | cct | resnet18 | wrn28_10")
+    parser.add_argument("--loss", type=str, default="crossentropy",
+                        help="crossentropy | linear_crossentropy (transformers:"
+                             " computed without the logits)")
+    parser.add_argument("--fused_norm", action="store_true", default=False,
+                        help="cct: layer norms on the framework's kernels")
+    parser.add_argument("--act_bits", type=int, default=32,
+                        help="cct: bits of the activations kept for the "
+                             "backward pass, 32 or 8")
     parser.add_argument("--engine", type=str, default="auto",
                         help="auto | loop")
     parser.add_argument("--no_hip_graphs", action="store_true", default=False)

@@ -1,0 +1,222 @@
+"""The token operators where the framework uses them: the transformers'
+layers, the simulator's logit-free loss, and a whole step of them together."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from blades_amd import Simulator, ops
+from blades_amd.models import CCT, MLP, get_model
+from blades_amd.models.layers import Act8Linear, FusedLayerNorm
+from blades_amd.models.text_cct import text_cct_2, text_transformer_2
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+QUIET = dict(dropout=0.0, attn_dropout=0.0, stochastic_depth=0.0)
+
+
+def text_model(**kw):
+    return text_cct_2(seq_len=12, vocab_size=60, num_classes=60,
+                      word_embedding_dim=24, **QUIET, **kw)
+
+
+def image_model(**kw):
+    return CCT(img_size=16, embedding_dim=32, num_layers=2, num_heads=2,
+               num_classes=10, **QUIET, **kw)
+
+
+def batch(model, device, n=6, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    if isinstance(model, CCT):
+        x = torch.randn(n, 3, 16, 16, generator=g)
+        y = torch.randint(0, 10, (n,), generator=g)
+    else:
+        x = torch.randint(1, 60, (n, 12), generator=g)
+        x[0, 5:] = 0                                   # padding
+        y = torch.randint(0, 60, (n,), generator=g)
+    return x.to(device), y.to(device)
+
+
+def grads_of(loss, model):
+    return torch.autograd.grad(loss, [p for p in model.parameters()])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("make", [text_model, image_model])
+def test_fused_norm_and_head_loss_match(device, make):
+    """Same state dict, same outputs and gradients as the torch layers."""
+    torch.manual_seed(0)
+    plain = make().to(device)
+    fused = make(fused_norm=True).to(device)
+    fused.load_state_dict(plain.state_dict())
+    assert any(isinstance(m, FusedLayerNorm) for m in fused.modules())
+    x, y = batch(plain, device)
+    torch.testing.assert_close(fused(x), plain(x), rtol=1e-4, atol=1e-5)
+    a = grads_of(F.cross_entropy(plain(x), y), plain)
+    loss = fused(x, targets=y)
+    torch.testing.assert_close(loss, F.cross_entropy(plain(x), y),
+                               rtol=1e-5, atol=1e-6)
+    for p, q in zip(a, grads_of(loss, fused)):
+        torch.testing.assert_close(q, p, rtol=1e-3, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("make", [text_model, image_model])
+def test_act8_models(device, make):
+    """Outputs are the torch layers'; gradients move by what 8-bit inputs
+    move them: a kept value is off by at most 2^-7 of its block's largest
+    (half a step of max / 63.5), so a layer's gradient is off by about that
+    share of its own size."""
+    torch.manual_seed(0)
+    plain = make().to(device)
+    act8 = make(act_bits=8).to(device)
+    act8.load_state_dict(plain.state_dict())
+    assert any(isinstance(m, Act8Linear) for m in act8.modules())
+    x, y = batch(plain, device)
+    torch.testing.assert_close(act8(x), plain(x), rtol=1e-4, atol=1e-5)
+    a = grads_of(F.cross_entropy(plain(x), y), plain)
+    b = grads_of(F.cross_entropy(act8(x), y), act8)
+    for (name, _), p, q in zip(plain.named_parameters(), a, b):
+        assert (p - q).norm() <= 0.05 * p.norm() + 1e-6, name
+
+
+def test_act_bits_refused():
+    with pytest.raises(ValueError):
+        image_model(act_bits=4)
+
+
+def test_registry_takes_the_options():
+    m = get_model("vit_lite", fused_norm=True, act_bits=8)
+    assert any(isinstance(s, Act8Linear) for s in m.modules())
+    assert m(torch.randn(1, 3, 32, 32)).shape == (1, 10)
+
+
+class TokenDataset:
+    """Next-word data of a few clients: (ids, the word to come)."""
+
+    def __init__(self, clients=4, steps=2, n=6, seed=0, device="cpu"):
+        g = torch.Generator().manual_seed(seed)
+        self.data = {}
+        for c in range(clients):
+            self.data[c] = [
+                (torch.randint(1, 60, (n, 12), generator=g).to(device),
+                 torch.randint(0, 60, (n,), generator=g).to(device))
+                for _ in range(steps)]
+
+    def get_clients(self):
+        return list(self.data)
+
+    def get_train_data(self, u, num_batches):
+        return self.data[u][:num_batches]
+
+    def get_stacked_train_data(self, ids, steps, device=None):
+        return [tuple(torch.stack([self.data[u][s][i] for u in ids]).to(device)
+                      for i in range(2)) for s in range(steps)]
+
+    def get_all_test_data(self, u):
+        x, y = self.data[u][0]
+        return torch.utils.data.TensorDataset(x.cpu(), y.cpu())
+
+
+def run_simulation(tmp_path, engine, device="cpu", rounds=2, steps=2,
+                   graphs=False, loss="linear_crossentropy", attack=None,
+                   **kw):
+    torch.manual_seed(0)
+    ds = TokenDataset(device=device)
+    sim = Simulator(ds, aggregator="mean", engine=engine, seed=3,
+                    num_byzantine=1 if attack else 0, attack=attack,
+                    log_path=str(tmp_path / f"{engine}{device}{graphs}{loss}"),
+                    use_cuda=device == "cuda", hip_graphs=graphs)
+    sim.run(text_model(**kw), loss=loss, global_rounds=rounds,
+            local_steps=steps, client_lr=0.05, server_lr=1.0,
+            validate_interval=1)
+    return sim.server.flat_parameters().cpu(), sim
+
+
+@pytest.mark.parametrize("attack", [None, "signflipping"])
+@pytest.mark.parametrize("kw", [{}, {"fused_norm": True, "act_bits": 8}])
+def test_fused_engine_matches_loop(tmp_path, kw, attack):
+    a, _ = run_simulation(tmp_path, "auto", attack=attack, **kw)
+    b, _ = run_simulation(tmp_path, "loop", attack=attack, **kw)
+    # the same sums in another order; an 8-bit rounding may fall the other
+    # way on such a difference, which moves a gradient by a step of 2^-6
+    tol = 1e-3 if kw else 1e-5
+    assert (a - b).abs().max() <= tol
+
+
+def test_head_loss_matches_crossentropy(tmp_path):
+    a, _ = run_simulation(tmp_path, "auto")
+    b, _ = run_simulation(tmp_path, "auto", loss="crossentropy")
+    torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
+
+
+def test_head_loss_refused_for_other_models(tmp_path):
+    ds = TokenDataset()
+    sim = Simulator(ds, aggregator="mean", log_path=str(tmp_path))
+    with pytest.raises(ValueError, match="linear_crossentropy"):
+        sim.run(MLP(), loss="linear_crossentropy", global_rounds=1)
+    with pytest.raises(NotImplementedError):
+        sim.run(MLP(), loss="hinge", global_rounds=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, {"fused_norm": True, "act_bits": 8}])
+def test_gpu_rounds_match_cpu(tmp_path, kw):
+    a, _ = run_simulation(tmp_path, "auto", "cuda", **kw)
+    b, _ = run_simulation(tmp_path, "auto", "cpu", **kw)
+    assert (a - b).abs().max() <= (2e-3 if kw else 1e-4)
+
+
+@pytest.mark.gpu
+def test_captured_rounds_match_eager(tmp_path):
+    """Rounds in one captured graph against eager ones; steps=1 trains on
+    shared parameters, steps=2 on each client's own."""
+    kw = {"fused_norm": True, "act_bits": 8}
+    for steps in (1, 2):
+        a, sim = run_simulation(tmp_path, "auto", "cuda", rounds=5,
+                                steps=steps, graphs=True, **kw)
+        b, _ = run_simulation(tmp_path, "auto", "cuda", rounds=5, steps=steps,
+                              **kw)
+        assert sim._graph_round is not None, "the round was not captured"
+        assert (a - b).abs().max() <= 1e-3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_operators_together(device, dtype):
+    """norm -> 8-bit linear -> 8-bit GELU -> 8-bit linear -> norm -> loss for
+    a population of clients, against 64-bit autograd per client.  The chain's
+    tolerance is the 8-bit steps': each kept tensor is off by at most 2^-7 of
+    its block's largest value, and bf16 adds 2^-8 a step."""
+    C, n, d, h, v = 3, 40, 48, 96, 130
+    g = torch.Generator().manual_seed(0)
+
+    def rnd(*s, scale=1.0):
+        return (torch.randn(*s, generator=g) * scale).to(device)
+    p = [rnd(d) * 0.1 + 1, rnd(d), rnd(h, d, scale=d ** -0.5), rnd(h),
+         rnd(d, h, scale=h ** -0.5), rnd(d), rnd(v, d, scale=d ** -0.5),
+         rnd(v)]
+    p = [t.to(dtype) for t in p]
+    x = rnd(C, n, d).to(dtype)
+    y = torch.randint(0, v, (C, n), generator=g).to(device)
+    y[1, :7] = -100
+
+    def own(p, x, y):
+        a = ops.layer_norm(x, p[0], p[1])
+        z = x + ops.linear_act8(ops.gelu_act8(ops.linear_act8(a, p[2], p[3])),
+                                p[4], p[5])
+        return ops.linear_cross_entropy(ops.layer_norm(z), p[6], y, p[7])
+
+    def plain(p, x, y):
+        a = F.layer_norm(x, (d,), p[0], p[1])
+        z = x + F.linear(F.gelu(F.linear(a, p[2], p[3])), p[4], p[5])
+        return F.cross_entropy(F.linear(F.layer_norm(z, (d,)), p[6], p[7]), y)
+
+    grads, loss = torch.func.vmap(torch.func.grad_and_value(own),
+                                  in_dims=(None, 0, 0))(tuple(p), x, y)
+    for c in range(C):
+        leaves = [t.detach().double().cpu().requires_grad_() for t in p]
+        ref = plain(leaves, x[c].double().cpu(), y[c].cpu())
+        want = torch.autograd.grad(ref, leaves)
+        assert abs(loss[c].cpu().double() - ref) <= 0.02 * ref
+        for a, r in zip(grads, want):
+            a = a[c].double().cpu()
+            assert (a - r).norm() <= 0.05 * r.norm()
