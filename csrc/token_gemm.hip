@@ -34,20 +34,25 @@ constexpr int kThreads = 256;          // of the small kernels below
 
 enum Src { F32, BF16, ACT8 };
 enum Epi { STORE, LSE, GRAD };
+enum Size { TINY, SMALL, LARGE };
 
 template <Src S> struct SrcOf;
 template <> struct SrcOf<F32> { using T = float; static constexpr int P = 3; };
 template <> struct SrcOf<BF16> { using T = bf16; static constexpr int P = 1; };
 template <> struct SrcOf<ACT8> { using T = int8_t; static constexpr int P = 1; };
 
-// Waves of a block along m and n, and each wave's 32 x 32 tiles.
-template <int WM_, int WN_, int MF_, int NF_, int BK_> struct Shape {
-  static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, BK = BK_;
+// Waves of a block along m and n, each wave's 32 x 32 tiles, and the depth of
+// a step for one-part and for three-part operands.
+template <int WM_, int WN_, int MF_, int NF_, int BK1_, int BK3_>
+struct Shape {
+  static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_;
+  static constexpr int BK1 = BK1_, BK3 = BK3_;
   static constexpr int BM = WM * MF * 32, BN = WN * NF * 32;
   static constexpr int THREADS = WM * WN * 64;
 };
-using Small = Shape<2, 2, 2, 2, 64>;       // 128 x 128, 4 waves
-using Large = Shape<2, 4, 4, 2, 64>;       // 256 x 256, 8 waves
+using Tiny = Shape<2, 2, 1, 1, 64, 32>;    // 64 x 64, 4 waves
+using Small = Shape<2, 2, 2, 2, 64, 16>;   // 128 x 128, 4 waves
+using Large = Shape<2, 4, 4, 2, 64, 16>;   // 256 x 256, 8 waves
 
 // What a kernel knows of an operand: `rows` of the output it feeds (m or n),
 // and how far the contiguous axis may be read.
@@ -250,7 +255,7 @@ struct Loader {
       int at;
       if constexpr (KM) {
         const int k = id / (ROWS / 8), c = id % (ROWS / 8);
-        at = k * ROWS + (((c >> 1) ^ (2 * (k & 3))) << 4) + (c & 1) * 8;
+        at = k * ROWS + (((c >> 1) ^ swap(k)) << 4) + (c & 1) * 8;
       } else {
         const int r = id / (BK / 8), c = id % (BK / 8);
         at = r * BK + ((c ^ swizzle(r)) << 3);
@@ -296,6 +301,12 @@ struct Loader {
     return r / (16 / C) % C;
   }
 
+  // 32-byte columns of a [BK][m] row likewise by k, so that the 4 rows and 2
+  // columns of a transposing read touch each bank once; k + 4 goes as k does.
+  static __device__ __forceinline__ int swap(int k) {
+    return ROWS >= 128 ? 2 * (k & 3) : 2 * ((k >> 1) & 1);
+  }
+
   // Fragment of the 32 rows from `base`, contraction step ks of 16.
   static __device__ __forceinline__ bf16x8 frag(const bf16* lds, int base,
                                                 int ks) {
@@ -306,7 +317,7 @@ struct Loader {
       const int c = (base >> 4) + ((lane >> 4) & 1);
       const int k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
       // k and k + 4 have the same low bits, so the same swizzle
-      const bf16* q = lds + k * ROWS + ((c ^ (2 * (k & 3))) << 4)
+      const bf16* q = lds + k * ROWS + ((c ^ swap(k)) << 4)
           + (i & 3) * 4;
       union { s4 h[2]; bf16x8 v; } u;
       typedef __attribute__((address_space(3))) s4* lds_s4;
@@ -341,9 +352,10 @@ __global__ __launch_bounds__(H::THREADS)
 void gemm_kernel(Params p) {
   constexpr int PA = SrcOf<SA>::P, PB = SrcOf<SB>::P;
   constexpr int MF = H::MF, NF = H::NF;
-  constexpr int BK = (PA == 3 || PB == 3) ? 16 : H::BK;
-  // a step of fp32 is short against memory's latency: two are on their way
-  constexpr int SETS = BK == 16 ? 2 : 1;
+  constexpr int BK = (PA == 3 || PB == 3) ? H::BK3 : H::BK1;
+  // a step of fp32 or of a tiny tile is short against memory's latency: two
+  // are on their way
+  constexpr int SETS = BK == H::BK3 || H::MF == 1 ? 2 : 1;
   using LA = Loader<SA, KMA, H::BM, H::THREADS, BK, SETS>;
   using LB = Loader<SB, KMB, H::BN, H::THREADS, BK, SETS>;
   __shared__ __attribute__((aligned(16))) bf16 sa[2][PA * LA::PLANE];
@@ -843,52 +855,58 @@ void launch_as(Params& p, long long groups, hipStream_t s) {
 }
 
 template <Src SA, bool KMA, Src SB, bool KMB, Epi E>
-void launch(Params& p, long long groups, bool large, hipStream_t s) {
-  if (large)
+void launch(Params& p, long long groups, Size size, hipStream_t s) {
+  if (size == LARGE)
     launch_as<SA, KMA, SB, KMB, Large, E>(p, groups, s);
-  else
+  else if (size == SMALL)
     launch_as<SA, KMA, SB, KMB, Small, E>(p, groups, s);
+  else
+    launch_as<SA, KMA, SB, KMB, Tiny, E>(p, groups, s);
 }
 
-// Large or small tiles, and parts of the contraction, by an estimate of the
-// time.  A compute unit works off blocks in rounds, one large or two small at
-// once.  A round's time is its area and its depth plus a fixed part (filling
-// the pipeline, the epilogue), which one large block alone does not hide as
-// well; measured: large tiles are 1.16 times as fast in the long run (bf16
-// 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
-// contractions (fp32 16 x 500 x 5000 x 300: 171 against 197 us) and where
-// few blocks would leave units idle.
+// Tile shape and parts of the contraction, by an estimate of the time.  A
+// compute unit works off blocks in rounds: one large, two small or three tiny
+// at once.  A round's time is its area and its depth plus a fixed part
+// (filling the pipeline, the epilogue), which a large block alone does not
+// hide as well.  Measured: large tiles are 1.16 times as fast in the long run
+// (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
+// contractions (fp32 16 x 500 x 5000 x 300: 171 against 197 us), tiny ones
+// where few blocks would leave units idle (fp32 2048 x 128 x 128: 8.7 against
+// 19.7 us).
 struct Tiling {
-  bool large;
+  Size size;
   int splits;
 };
+const int kTileM[3] = {Tiny::BM, Small::BM, Large::BM};
+const int kTileN[3] = {Tiny::BN, Small::BN, Large::BN};
 
 // `deep`: whether the contraction may be cut into parts, each at least 256
 // deep.  `products`: matrix instructions per multiplication (1, 3 or 6).
 Tiling tiling(long long groups, long long m, long long n, long long k,
               bool deep, int products) {
-  Tiling best = {false, 1};
-  double least = -1;
+  // rounds with up to 256 blocks (one a compute unit), and full ones
+  const int slots[3] = {768, 512, 256};
+  const double alone[3] = {0.5, 1.4, 4.0}, full[3] = {1.12, 2.32, 4.0};
+  const double fixed[3] = {60, 50, 92};
   // 128 x 128 x 1 steps of a compute unit per microsecond
   const double rate = products == 6 ? 24 : products == 3 ? 45 : 135;
   const long long most = deep ? std::max<long long>(
       1, std::min<long long>(k / 256, 64)) : 1;
-  for (int large = 0; large < 2; ++large) {
-    const long long bm = large ? Large::BM : Small::BM;
-    const long long bn = large ? Large::BN : Small::BN;
-    const long long tiles = ceil_div(m, bm) * ceil_div(n, bn) * groups;
+  Tiling best = {SMALL, 1};
+  double least = -1;
+  for (int z = 0; z < 3; ++z) {
+    const long long tiles =
+        ceil_div(m, kTileM[z]) * ceil_div(n, kTileN[z]) * groups;
     for (long long splits = 1; splits <= most; ++splits) {
-      const long long blocks = tiles * splits;
-      const double rounds = large
-          ? 4.0 * ceil_div(blocks, 256)
-          : 2.32 * (blocks / 512)
-              + (blocks % 512 == 0 ? 0 : blocks % 512 <= 256 ? 1.4 : 2.32);
-      double us = rounds * (ceil_div(k, splits) + (large ? 92 : 50)) / rate;
+      const long long blocks = tiles * splits, rest = blocks % slots[z];
+      const double rounds = full[z] * (blocks / slots[z])
+          + (rest == 0 ? 0 : rest <= 256 ? alone[z] : full[z]);
+      double us = rounds * (ceil_div(k, splits) + fixed[z]) / rate;
       // the parts are written, read and joined
       if (splits > 1) us += 4 + (2 * splits + 1) * 4e-6 * m * n * groups / 4;
       if (least < 0 || us < least) {
         least = us;
-        best = {large != 0, (int)splits};
+        best = {(Size)z, (int)splits};
       }
     }
   }
@@ -927,21 +945,21 @@ void gemm(const Gemm& g, hipStream_t s) {
   p.partial = g.partial;
   p.scale = g.scale;
   const bool f = g.ta == kF32;
-  const bool large = tiling(g.groups, g.m, g.n, g.k, true,
-                            products_of(g.ta, g.b.e != nullptr)).large;
+  const Size size = tiling(g.groups, g.m, g.n, g.k, true,
+                           products_of(g.ta, g.b.e != nullptr)).size;
   const long long n = g.groups;
   if (g.b.e) {                                     // dY' X8
-    if (f) launch<F32, true, ACT8, true, STORE>(p, n, large, s);
-    else launch<BF16, true, ACT8, true, STORE>(p, n, large, s);
+    if (f) launch<F32, true, ACT8, true, STORE>(p, n, size, s);
+    else launch<BF16, true, ACT8, true, STORE>(p, n, size, s);
   } else if (!g.a_kmajor && !g.b_kmajor) {         // X W'
-    if (f) launch<F32, false, F32, false, STORE>(p, n, large, s);
-    else launch<BF16, false, BF16, false, STORE>(p, n, large, s);
+    if (f) launch<F32, false, F32, false, STORE>(p, n, size, s);
+    else launch<BF16, false, BF16, false, STORE>(p, n, size, s);
   } else if (!g.a_kmajor) {                        // dY W
-    if (f) launch<F32, false, F32, true, STORE>(p, n, large, s);
-    else launch<BF16, false, BF16, true, STORE>(p, n, large, s);
+    if (f) launch<F32, false, F32, true, STORE>(p, n, size, s);
+    else launch<BF16, false, BF16, true, STORE>(p, n, size, s);
   } else {                                         // P' W, P stored by word
-    if (f) launch<F32, true, F32, true, STORE>(p, n, large, s);
-    else launch<BF16, true, BF16, true, STORE>(p, n, large, s);
+    if (f) launch<F32, true, F32, true, STORE>(p, n, size, s);
+    else launch<BF16, true, BF16, true, STORE>(p, n, size, s);
   }
 }
 
@@ -961,11 +979,13 @@ void join_partials(const float* partial, int splits, long long groups,
         out_group, static_cast<const bf16*>(bias), bias_group);
 }
 
+static Size loss_size(const Loss& l) {
+  return tiling(l.groups, l.vocab, l.rows, l.dim, false,
+                products_of(l.t, false)).size;
+}
 void loss_tile(const Loss& l, int* m, int* n) {
-  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
-                            products_of(l.t, false)).large;
-  *m = large ? Large::BM : Small::BM;
-  *n = large ? Large::BN : Small::BN;
+  *m = kTileM[loss_size(l)];
+  *n = kTileN[loss_size(l)];
 }
 long long loss_sum_blocks(long long rows) { return ceil_div(rows, 32); }
 
@@ -994,10 +1014,9 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
   Params p = loss_params(l, 0, l.vocab);
   p.part = static_cast<float2*>(part);
   p.picked = picked;
-  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
-                            products_of(l.t, false)).large;
-  if (l.t == kF32) launch<F32, false, F32, false, LSE>(p, l.groups, large, s);
-  else launch<BF16, false, BF16, false, LSE>(p, l.groups, large, s);
+  const Size size = loss_size(l);
+  if (l.t == kF32) launch<F32, false, F32, false, LSE>(p, l.groups, size, s);
+  else launch<BF16, false, BF16, false, LSE>(p, l.groups, size, s);
   const long long blocks = loss_sum_blocks(l.rows);
   lse_kernel<<<dim3(grid_of(blocks), (unsigned)l.groups), kThreads, 0, s>>>(
       p.part, picked, l.target, l.ignore, l.vocab, p.tiles_m, l.rows, lse,
@@ -1016,10 +1035,9 @@ void loss_logit_grad(const Loss& l, long long v0, long long nv,
   p.out = pt;
   p.out_ld = pt_ld;
   p.out_group = pt_group;
-  const bool large = tiling(l.groups, l.vocab, l.rows, l.dim, false,
-                            products_of(l.t, false)).large;
-  if (l.t == kF32) launch<F32, false, F32, false, GRAD>(p, l.groups, large, s);
-  else launch<BF16, false, BF16, false, GRAD>(p, l.groups, large, s);
+  const Size size = loss_size(l);
+  if (l.t == kF32) launch<F32, false, F32, false, GRAD>(p, l.groups, size, s);
+  else launch<BF16, false, BF16, false, GRAD>(p, l.groups, size, s);
 }
 
 void row_scale(const float* grad, long long groups, long long rows,
