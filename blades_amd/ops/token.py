@@ -312,6 +312,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     (target's shape), ``"sum"``, or ``"mean"`` over the rows that count (NaN
     where none does, as torch has it; their gradient is zero).
 
+    In float32 a value of ``x`` or ``weight`` that is not finite makes the
+    results it enters NaN.
+
     A target outside the vocabulary cannot raise without stopping the GPU's
     stream: its row's loss, and every gradient it enters, is NaN.  ``bias``
     may hold -inf for words that are switched off.
@@ -390,7 +393,8 @@ def gelu_act8(x: Tensor) -> Tensor:
     Along the last axis every 128 values share the least power of two
     ``2**e`` (e >= -126) with ``max|x| <= 127 * 2**e`` and are held as int8:
     1.008 bytes a value.  The gradient is the formula's at the values held,
-    which differ from ``x`` by at most ``2**(e-1)``; a block of 128 that
+    which differ from ``x`` by at most ``2**(e-1)`` (what would round to
+    2**128 is held as 63 * 2**122); a block of 128 that
     holds an infinity or NaN has gradient NaN.  The output comes from ``x``
     itself.
     """
@@ -506,11 +510,14 @@ def linear_act8(x: Tensor, weight: Tensor,
     held are used as they are in that product.  ``weight``: [out, in];
     ``bias``: [out] or None.
 
-    In float32 a value that is not finite makes the results it enters NaN.
+    In float32 a value that is not finite makes the results it enters NaN,
+    and magnitudes below 2**-110 lose low bits.
     """
     _check_input("x", x)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be an [out, in] tensor")
+    if weight.shape[0] == 0:
+        raise ValueError("weight has no rows")
     _check_param("weight", weight, x, (weight.shape[0], x.shape[-1]))
     _check_param("bias", bias, x, weight.shape[:1])
     ext = _extension(x)

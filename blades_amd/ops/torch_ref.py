@@ -263,6 +263,9 @@ def act8_pack(x: Tensor):
     e = (k - 7 + (m > 127.0 / 128.0).int()).clamp(min=-126)
     e = torch.where(top == 0, torch.full_like(e, -126), e)
     q = torch.round(torch.ldexp(blocks, -e))
+    # 64 units of the largest exponent would be 2^128, beyond float32
+    most = torch.where(e == 122, 63.0, 127.0)
+    q = torch.minimum(torch.maximum(q, -most), most)
     q = torch.where(finite, q, torch.zeros_like(q)).to(torch.int8)
     code = torch.where(finite, e + 127, torch.full_like(e, 255))
     return (q.reshape(*x.shape[:-1], n + pad)[..., :n].contiguous(),

@@ -5,7 +5,8 @@
 // nearest integer (ties to even).  A power of two makes the scaling exact:
 // the one rounding is the integer's, at most half a step of max|x| / 63.5,
 // and the stored value is exact in bfloat16, so a matrix product can take it
-// as it is.  (8-bit floats would spend bits on range that a block of 128
+// as it is.  A value that would round to 2^128 is held as 63 * 2^122.
+// (8-bit floats would spend bits on range that a block of 128
 // activations does not have: on normal data their error is 2 to 4 times
 // larger.)  A block with an infinity or NaN reads back as NaN.
 //
@@ -84,13 +85,16 @@ __device__ __forceinline__ void pack8(const float (&v)[8], uint32_t& e,
     top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   e = block_exponent(top);
   const float inv = e == 255u ? 0.f : __uint_as_float((254u - e) << 23);
+  // under the largest exponent 64 units would be 2^128, beyond fp32
+  const float most = e == 249u ? 63.f : 127.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // a block that is not finite stores zeros: 0 * inf reads back as NaN
-      const int n = e == 255u ? 0 : (int)rintf(v[4 * h + j] * inv);
+      const float r = fminf(fmaxf(rintf(v[4 * h + j] * inv), -most), most);
+      const int n = e == 255u ? 0 : (int)r;
       w |= (uint32_t)(n & 0xff) << (8 * j);
     }
     q[h] = w;

@@ -60,71 +60,71 @@ void norm_fwd_kernel(NormArgs a) {
   // a row slot's threads leave the loop together, a block's for TPR == 256
   for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
        row < total; row += (long long)gridDim.x * RPB) {
-  const long long g = a.groups == 1 ? 0 : row / a.rows;
-  const T* x = static_cast<const T*>(a.x) + row * a.dim;
+    const long long g = a.groups == 1 ? 0 : row / a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.dim;
 
-  float v[NV][VEC];
-  float s[2] = {0.f, 0.f};
+    float v[NV][VEC];
+    float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + lane) * VEC;
-    if (c < dim) {
-      load_n<VEC>(x + c, v[i]);
-    } else {
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < dim) {
+        load_n<VEC>(x + c, v[i]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+        for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
     }
+    float one[1] = {s[0]};
+    row_sum<TPR, 1>(one, red);
+    const float inv = 1.f / (float)dim;
+    float mean = one[0] * inv;
+    // The centred values' own mean corrects what the first sum rounded away,
+    // which matters where the mean is large against the deviation.
+    s[0] = s[1] = 0.f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
-  }
-  float one[1] = {s[0]};
-  row_sum<TPR, 1>(one, red);
-  const float inv = 1.f / (float)dim;
-  float mean = one[0] * inv;
-  // The centred values' own mean corrects what the first sum rounded away,
-  // which matters where the mean is large against the deviation.
-  s[0] = s[1] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < dim) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + lane) * VEC;
-    if (c < dim) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = v[i][j] - mean;
-        s[0] += d;
-        s[1] += d * d;
+        for (int j = 0; j < VEC; ++j) {
+          const float d = v[i][j] - mean;
+          s[0] += d;
+          s[1] += d * d;
+        }
       }
     }
-  }
-  row_sum<TPR, 2>(s, red);
-  const float off = s[0] * inv;
-  const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
-  mean += off;
+    row_sum<TPR, 2>(s, red);
+    const float off = s[0] * inv;
+    const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
+    mean += off;
 
-  const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
-  const T* b = a.b ? static_cast<const T*>(a.b) + g * a.b_stride : nullptr;
-  T* y = static_cast<T*>(a.y) + row * a.dim;
+    const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
+    const T* b = a.b ? static_cast<const T*>(a.b) + g * a.b_stride : nullptr;
+    T* y = static_cast<T*>(a.y) + row * a.dim;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + lane) * VEC;
-    if (c < dim) {
-      float wv[VEC], bv[VEC];
-      if (w) load_n<VEC>(w + c, wv);
-      if (b) load_n<VEC>(b + c, bv);
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < dim) {
+        float wv[VEC], bv[VEC];
+        if (w) load_n<VEC>(w + c, wv);
+        if (b) load_n<VEC>(b + c, bv);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float h = (v[i][j] - mean) * rstd;
-        if (w) h *= wv[j];
-        if (b) h += bv[j];
-        v[i][j] = h;
+        for (int j = 0; j < VEC; ++j) {
+          float h = (v[i][j] - mean) * rstd;
+          if (w) h *= wv[j];
+          if (b) h += bv[j];
+          v[i][j] = h;
+        }
+        store_n<VEC>(y + c, v[i]);
       }
-      store_n<VEC>(y + c, v[i]);
     }
-  }
-  if (lane == 0) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
+    if (lane == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
   }
 }
 
@@ -261,34 +261,34 @@ void norm_fwd_wide_kernel(NormArgs a) {
   __shared__ float red[8];
   for (long long row = blockIdx.x; row < a.groups * a.rows;
        row += gridDim.x) {
-  const long long g = row / a.rows;
-  const T* x = static_cast<const T*>(a.x) + row * a.dim;
-  const float inv = 1.f / (float)a.dim;
-  float one[1] = {0.f};
-  for (long long c = threadIdx.x; c < a.dim; c += kThreads)
-    one[0] += to_f(x[c]);
-  row_sum<256, 1>(one, red);
-  float mean = one[0] * inv;
-  float s[2] = {0.f, 0.f};
-  for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
-    const float d = to_f(x[c]) - mean;
-    s[0] += d;
-    s[1] += d * d;
-  }
-  row_sum<256, 2>(s, red);
-  const float off = s[0] * inv;
-  const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
-  mean += off;
-  const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
-  const T* b = a.b ? static_cast<const T*>(a.b) + g * a.b_stride : nullptr;
-  T* y = static_cast<T*>(a.y) + row * a.dim;
-  for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
-    float h = (to_f(x[c]) - mean) * rstd;
-    if (w) h *= to_f(w[c]);
-    if (b) h += to_f(b[c]);
-    y[c] = from_f<T>(h);
-  }
-  if (threadIdx.x == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
+    const long long g = row / a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.dim;
+    const float inv = 1.f / (float)a.dim;
+    float one[1] = {0.f};
+    for (long long c = threadIdx.x; c < a.dim; c += kThreads)
+      one[0] += to_f(x[c]);
+    row_sum<256, 1>(one, red);
+    float mean = one[0] * inv;
+    float s[2] = {0.f, 0.f};
+    for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float d = to_f(x[c]) - mean;
+      s[0] += d;
+      s[1] += d * d;
+    }
+    row_sum<256, 2>(s, red);
+    const float off = s[0] * inv;
+    const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
+    mean += off;
+    const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
+    const T* b = a.b ? static_cast<const T*>(a.b) + g * a.b_stride : nullptr;
+    T* y = static_cast<T*>(a.y) + row * a.dim;
+    for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
+      float h = (to_f(x[c]) - mean) * rstd;
+      if (w) h *= to_f(w[c]);
+      if (b) h += to_f(b[c]);
+      y[c] = from_f<T>(h);
+    }
+    if (threadIdx.x == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
   }
 }
 
@@ -298,27 +298,27 @@ void norm_bwd_wide_kernel(NormArgs a) {
   __shared__ float red[8];
   for (long long row = blockIdx.x; row < a.groups * a.rows;
        row += gridDim.x) {
-  const long long g = row / a.rows;
-  const T* x = static_cast<const T*>(a.x) + row * a.dim;
-  const T* dy = static_cast<const T*>(a.dy) + row * a.dim;
-  const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
-  T* dx = static_cast<T*>(a.y) + row * a.dim;
-  const float mean = a.mean[row], rstd = a.rstd[row];
-  float s[2] = {0.f, 0.f};
-  for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
-    const float h = (to_f(x[c]) - mean) * rstd;
-    const float d = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
-    s[0] += d;
-    s[1] += d * h;
-  }
-  row_sum<256, 2>(s, red);
-  const float inv = 1.f / (float)a.dim;
-  const float c1 = s[0] * inv, c2 = s[1] * inv;
-  for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
-    const float h = (to_f(x[c]) - mean) * rstd;
-    const float d = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
-    dx[c] = from_f<T>(rstd * (d - c1 - h * c2));
-  }
+    const long long g = row / a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.dim;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dim;
+    const T* w = a.w ? static_cast<const T*>(a.w) + g * a.w_stride : nullptr;
+    T* dx = static_cast<T*>(a.y) + row * a.dim;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float h = (to_f(x[c]) - mean) * rstd;
+      const float d = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
+      s[0] += d;
+      s[1] += d * h;
+    }
+    row_sum<256, 2>(s, red);
+    const float inv = 1.f / (float)a.dim;
+    const float c1 = s[0] * inv, c2 = s[1] * inv;
+    for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float h = (to_f(x[c]) - mean) * rstd;
+      const float d = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
+      dx[c] = from_f<T>(rstd * (d - c1 - h * c2));
+    }
   }
 }
 

@@ -846,6 +846,13 @@ struct LossNode : public TokenNode {            // x, w, target, b, lse, count
   }
 };
 
+template <typename... T>
+void refuse_forward_mode(const char* op, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !(torch::autograd::isFwGradDefined(inputs) || ...), op,
+      " has no forward-mode derivative");
+}
+
 template <typename N>
 std::shared_ptr<N> make_node(torch::autograd::edge_list&& edges) {
   std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
@@ -857,6 +864,7 @@ Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
                    const OptTensor& b, double eps, int64_t groups) {
   std::shared_ptr<NormNode> node;
   const Tensor wt = or_undefined(w), bt = or_undefined(b);
+  refuse_forward_mode("layer_norm", x, w, b);
   if (torch::autograd::compute_requires_grad(x, wt, bt))
     node = make_node<NormNode>(torch::autograd::collect_next_edges(x, wt, bt));
   Int3 out;
@@ -877,6 +885,7 @@ Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
 // it (the call on a vmap's whole population) must not drop it.
 Int3 gelu_autograd(c10::DispatchKeySet ks, const Tensor& x, bool keep) {
   std::shared_ptr<GeluNode> node;
+  refuse_forward_mode("gelu_act8", x);
   if (torch::autograd::compute_requires_grad(x))
     node = make_node<GeluNode>(torch::autograd::collect_next_edges(x));
   Int3 out;
@@ -896,6 +905,7 @@ Int3 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
                      const OptTensor& b, bool keep, int64_t groups) {
   std::shared_ptr<LinearNode> node;
   const Tensor bt = or_undefined(b);
+  refuse_forward_mode("linear_act8", x, w, b);
   if (torch::autograd::compute_requires_grad(x, w, bt))
     node =
         make_node<LinearNode>(torch::autograd::collect_next_edges(x, w, bt));
@@ -919,6 +929,7 @@ Int3 loss_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
                    int64_t reduction, int64_t groups) {
   std::shared_ptr<LossNode> node;
   const Tensor bt = or_undefined(b);
+  refuse_forward_mode("linear_cross_entropy", x, w, b);
   if (torch::autograd::compute_requires_grad(x, w, bt))
     node = make_node<LossNode>(torch::autograd::collect_next_edges(x, w, bt));
   Int3 out;

@@ -272,16 +272,17 @@ struct Loader {
       } else if constexpr (S == BF16) {
         o[0] = raw[i].v;
       } else {
-        // (q + 128) * unit - 128 * unit, exact: bytes convert unsigned
+        // Bytes convert unsigned; (q + 128) - 128 and its product with a
+        // power of two are exact.  (One fma with -128 * unit would overflow
+        // for blocks that reach 2^127.)
         const float unit = __uint_as_float(raw[i].e << 23);
-        const float off = -128.f * unit;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t w = raw[i].v[h] ^ 0x80808080u;
           float v[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            v[t] = fmaf((float)((w >> (8 * t)) & 0xffu), unit, off);
+            v[t] = ((float)((w >> (8 * t)) & 0xffu) - 128.f) * unit;
           o[0][2 * h] = __builtin_amdgcn_perm(
               __float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
           o[0][2 * h + 1] = __builtin_amdgcn_perm(
@@ -897,6 +898,8 @@ Tiling tiling(long long groups, long long m, long long n, long long k,
   for (int z = 0; z < 3; ++z) {
     const long long tiles =
         ceil_div(m, kTileM[z]) * ceil_div(n, kTileN[z]) * groups;
+    // tiny tiles of a huge output: too many blocks, and never the best
+    if (z == TINY && tiles > 1 << 16) continue;
     for (long long splits = 1; splits <= most; ++splits) {
       const long long blocks = tiles * splits, rest = blocks % slots[z];
       const double rounds = full[z] * (blocks / slots[z])

@@ -93,7 +93,9 @@ def stored64(x):
                     ~torch.isfinite(top)).all()):
                 break
         unit = torch.exp2(e)
+        # what would round to 2^128, beyond fp32, stays one unit below
         v = torch.round(part / unit) * unit
+        v = torch.where(v.abs() == 2.0 ** 128, v.sign() * 63 * 2.0 ** 122, v)
         out[..., lo:lo + 128] = torch.where(torch.isfinite(top), v,
                                             torch.full_like(v, math.nan))
     return out
@@ -594,6 +596,52 @@ def test_linear_wide_range(device):
                  rand(50, 20, device=device, seed=2, scale=1e-6))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n,m", [(1500, 77, 203), (700, 1025, 131),
+                                      (4100, 1030, 2051), (9000, 4, 3),
+                                      (5001, 520, 777)])
+def test_linear_long_and_odd(dtype, rows, n, m):
+    """Every tile size with rows that end inside a 16-byte access, and
+    contractions long enough for the unchecked steps."""
+    check_linear(rand(rows, n, dtype=dtype, device="cuda"),
+                 rand(m, n, dtype=dtype, device="cuda", seed=1),
+                 rand(m, dtype=dtype, device="cuda", seed=2),
+                 rand(rows, m, dtype=dtype, device="cuda", seed=3))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(1000, 333, 1001),
+                                            (2500, 77, 5003),
+                                            (64, 1030, 9999)])
+def test_loss_long_and_odd(dtype, rows, dim, vocab):
+    x, w, y, b = loss_inputs(rows, dim, vocab, dtype, "cuda")
+    check_loss(x, w, y, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_largest_values(device):
+    """8-bit blocks that reach fp32's largest values keep them."""
+    x = rand(30, 256, device=device).clamp(-1, 1)
+    x[:, :128] *= 3.3e38
+    x[4, 3], x[5, 4] = 3.4e38, -3.4e38
+    w = torch.zeros(20, 256, device=device)
+    check_linear(x, w, None, rand(30, 20, device=device, scale=1e-30))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", ["norm", "loss", "gelu", "linear"])
+def test_forward_mode_refused(device, fn):
+    x, w, y, b = loss_inputs(4, 16, 16, torch.float32, device)
+    call = {"norm": lambda x: ops.layer_norm(x, b, b),
+            "loss": lambda x: ops.linear_cross_entropy(x, w, y, b),
+            "gelu": ops.gelu_act8,
+            "linear": lambda x: ops.linear_act8(x, w, b)}[fn]
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_linear_no_rows(device):
     x = torch.empty(0, 8, device=device, requires_grad=True)
@@ -615,6 +663,8 @@ def test_act8_refusals():
         ops.gelu_act8(torch.tensor(1.0))
     with pytest.raises(ValueError):
         ops.linear_act8(x, torch.randn(8))
+    with pytest.raises(ValueError):
+        ops.linear_act8(x, torch.randn(0, 8))
     with pytest.raises(ValueError):
         ops.linear_act8(x, torch.randn(4, 7))
     with pytest.raises(ValueError):
