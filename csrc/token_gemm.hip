@@ -399,20 +399,22 @@ void gemm_kernel(Params p) {
 
   // Units of a step: one 16-deep slice of one row of the wave's tiles.
   constexpr int UNITS = BK / 16 * MF;
-  bf16x8 fb[NF][PB];
+  bf16x8 fbs[2][NF][PB];                 // of even and odd slices
   auto read_b = [&](const bf16* tb, int ks) {
 #pragma unroll
     for (int j = 0; j < NF; ++j)
 #pragma unroll
       for (int q = 0; q < PB; ++q)
-        fb[j][q] = LB::frag(tb + q * LB::PLANE, wn + j * 32, ks);
+        fbs[ks & 1][j][q] = LB::frag(tb + q * LB::PLANE, wn + j * 32, ks);
   };
   auto read_a = [&](const bf16* ta, int u, bf16x8 (&fa)[PA]) {
 #pragma unroll
     for (int q = 0; q < PA; ++q)
       fa[q] = LA::frag(ta + q * LA::PLANE, wm + u % MF * 32, u / MF);
   };
-  auto products = [&](int i, const bf16x8 (&fa)[PA]) {
+  auto products = [&](int u, const bf16x8 (&fa)[PA]) {
+    const int i = u % MF;
+    const bf16x8(&fb)[NF][PB] = fbs[u / MF & 1];
 #pragma unroll
     for (int qa = 0; qa < PA; ++qa)
 #pragma unroll
@@ -424,18 +426,16 @@ void gemm_kernel(Params p) {
               fa[qa], fb[j][qb], acc[i][j], 0, 0, 0);
       }
   };
-  auto multiply = [&](const bf16* ta, const bf16* tb, auto from) {
+  auto multiply = [&](const bf16* ta, const bf16* tb) {
 #pragma unroll
-    for (int u = from(); u < UNITS; ++u) {
+    for (int u = 0; u < UNITS; ++u) {
       if (u % MF == 0) read_b(tb, u / MF);
       bf16x8 fa[PA];
       read_a(ta, u, fa);
-      products(u % MF, fa);
+      products(u, fa);
     }
   };
   constexpr int FIRST = MF;      // units that cover conversion and writing
-  using First = std::integral_constant<int, FIRST>;
-  using None = std::integral_constant<int, 0>;
 
   // Two tiles in LDS: one is multiplied while the next is converted and
   // written, and the one or two after it are on their way in registers.  One
@@ -449,6 +449,11 @@ void gemm_kernel(Params p) {
     bf16x8 fa[FIRST][PA];
 #pragma unroll
     for (int u = 0; u < FIRST; ++u) read_a(sa[cur()], u, fa[u]);
+    bf16x8 ahead[2][PA];
+    if (UNITS > FIRST) {
+      read_b(sb[cur()], 1);
+      read_a(sa[cur()], FIRST, ahead[FIRST & 1]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     la.template store<decltype(set)::value>(sa[cur() ^ 1]);
     lb.template store<decltype(set)::value>(sb[cur() ^ 1]);
@@ -468,7 +473,17 @@ void gemm_kernel(Params p) {
     la.template load_whole<decltype(set)::value>();
     lb.template load_whole<decltype(set)::value>();
     __builtin_amdgcn_sched_barrier(0);
-    multiply(sa[cur()], sb[cur()], First());
+    // fragments are read one unit ahead of their products
+#pragma unroll
+    for (int u = FIRST; u < UNITS; ++u) {
+      if (u + 1 < UNITS) {
+        if ((u + 1) % MF == 0) read_b(sb[cur()], (u + 1) / MF);
+        read_a(sa[cur()], u + 1, ahead[(u + 1) & 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      products(u, ahead[u & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   auto checked_step = [&](int s, auto cur, auto set) {
     __syncthreads();
@@ -480,7 +495,7 @@ void gemm_kernel(Params p) {
       la.template load<decltype(set)::value>((s + 1 + SETS) * BK);
       lb.template load<decltype(set)::value>((s + 1 + SETS) * BK);
     }
-    multiply(sa[cur()], sb[cur()], None());
+    multiply(sa[cur()], sb[cur()]);
   };
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;
