@@ -350,7 +350,8 @@ void norm_params_wide_kernel(NormArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads)
 void join_rows_kernel(const float* __restrict__ partial, long long blocks,
-                      long long width, long long split, T* out0, T* out1) {
+                      long long width, long long split, T* out0,
+                      long long out0_group, T* out1, Scale scale) {
   __shared__ float part[8][33];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const long long c = (long long)blockIdx.x * 32 + cl;
@@ -374,8 +375,9 @@ void join_rows_kernel(const float* __restrict__ partial, long long blocks,
   if (rl == 0 && c < width) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += part[i][cl];
+    s *= scale_of(scale, g);
     if (c < split) {
-      if (out0) out0[g * split + c] = from_f<T>(s);
+      if (out0) out0[g * out0_group + c] = from_f<T>(s);
     } else if (out1) {
       out1[g * (width - split) + (c - split)] = from_f<T>(s);
     }
@@ -520,7 +522,8 @@ void backward_t(const NormArgs& a, hipStream_t s) {
     join_rows_kernel<T>
         <<<dim3((unsigned)ceil_div(2 * a.dim, 32), (unsigned)a.groups),
            kThreads, 0, s>>>(a.partial, blocks, 2 * a.dim, a.dim,
-                             static_cast<T*>(a.dw), static_cast<T*>(a.db));
+                             static_cast<T*>(a.dw), a.dim,
+                             static_cast<T*>(a.db), Scale{});
 }
 
 }  // namespace
@@ -571,13 +574,21 @@ void colsum(const void* x, void* out, float* partial, long long groups,
     else
       colsum_kernel<bf16, 1><<<grid, kThreads, 0, s>>>(p, partial, rows, cols);
   }
-  const dim3 jgrid((unsigned)ceil_div(cols, 32), (unsigned)groups);
+  join_rows(partial, groups, blocks, cols, out, cols, Scale{}, t, s);
+}
+
+void join_rows(const float* partial, long long groups, long long blocks,
+               long long cols, void* out, long long out_group,
+               const Scale& scale, DType t, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)groups);
   if (t == kF32)
-    join_rows_kernel<float><<<jgrid, kThreads, 0, s>>>(
-        partial, blocks, cols, cols, static_cast<float*>(out), nullptr);
+    join_rows_kernel<float><<<grid, kThreads, 0, s>>>(
+        partial, blocks, cols, cols, static_cast<float*>(out), out_group,
+        nullptr, scale);
   else
-    join_rows_kernel<bf16><<<jgrid, kThreads, 0, s>>>(
-        partial, blocks, cols, cols, static_cast<bf16*>(out), nullptr);
+    join_rows_kernel<bf16><<<grid, kThreads, 0, s>>>(
+        partial, blocks, cols, cols, static_cast<bf16*>(out), out_group,
+        nullptr, scale);
 }
 
 }  // namespace token_ops

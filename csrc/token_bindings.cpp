@@ -278,8 +278,9 @@ void run_gemm(Gemm& g, const Tensor& like) {
   g.partial = partial.data_ptr<float>();
   g.splits = splits;
   gemm(g, s);
-  join_partials(g.partial, splits, g.groups, g.m, g.n, g.out, g.out_ld,
-                g.out_group, g.bias, g.bias_group, g.tout, s);
+  TORCH_CHECK(g.out_ld == g.n, "a joined output's rows have no gaps");
+  join_partials(g.partial, splits, g.groups, g.m, g.n, g.out, g.out_group,
+                g.bias, g.bias_group, g.tout, s);
 }
 
 // y[g] = x[g] w' + b
@@ -522,11 +523,16 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
     scale.num = top.data_ptr<float>();
   }
 
+  Tensor bsum;
+  const long long parts_b = loss_row_parts(l);
+  if (want_b) bsum = floats(x, {l.groups, parts_b, std::min(piece, l.vocab)});
+
   for (long long v0 = 0; v0 < l.vocab; v0 += piece) {
     const long long nv = std::min(piece, l.vocab - v0);
     loss_logit_grad(l, v0, nv, lse.data_ptr<float>(),
                     reduction ? nullptr : ratio.data_ptr<float>(),
-                    pt.data_ptr(), ld, piece * ld, s);
+                    pt.data_ptr(), ld, piece * ld,
+                    want_b ? bsum.data_ptr<float>() : nullptr, s);
     Mat pm = mat(pt, piece * ld);
     pm.padded = true;
     if (want_x) {
@@ -560,13 +566,13 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
       run_gemm(g, x);
     }
     if (want_b)
-      rowsum(pt.data_ptr(), ld, piece * ld, l.groups, nv, ld,
-             static_cast<char*>(db.data_ptr()) + v0 * size, l.vocab, scale, l.t,
-             s);
+      join_rows(bsum.data_ptr<float>(), l.groups, parts_b, nv,
+                static_cast<char*>(db.data_ptr()) + v0 * size, l.vocab, scale,
+                l.t, s);
   }
   if (want_x && parts)
     join_partials(xsum.data_ptr<float>(), splits, l.groups, l.rows, l.dim,
-                  dx.data_ptr(), l.dim, l.rows * l.dim, nullptr, 0, l.t, s);
+                  dx.data_ptr(), l.rows * l.dim, nullptr, 0, l.t, s);
   return {dx, dw, db};
 }
 

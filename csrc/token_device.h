@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "token_ops.h"
+
 namespace token_ops {
 
 using bf16 = __bf16;
@@ -83,6 +85,13 @@ __device__ __forceinline__ void store_n(bf16* p, const float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = (bf16)v[i];
   }
+}
+
+__device__ __forceinline__ float scale_of(const Scale& s, long long g) {
+  if (!s.num) return 1.f;
+  if (!s.den) return s.num[g];
+  // nothing counted: nothing to scale
+  return s.den[g] == 0.f ? 0.f : s.num[g] / s.den[g];
 }
 
 // Sum over groups of W neighbouring lanes (W a power of two up to 64); every

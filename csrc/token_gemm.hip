@@ -12,14 +12,21 @@
 // multiplication have 2.6 times the rate of the fp32 matrix instruction.
 // A value that is not finite makes its results NaN (inf - inf in the parts).
 //
-// A block of 4 waves owns 128 x 128 of the output, each wave 64 x 64 in
-// v_mfma_f32_32x32x16_bf16 tiles.  Global loads of the next step are in
-// flight, in registers, while the current step multiplies out of LDS.
-//   [m][k] tiles lie in LDS as [128][BK] with 16-byte columns swizzled by the
+// A block owns 256 x 256, 128 x 128 or 64 x 64 of the output (tiling() below
+// chooses) in v_mfma_f32_32x32x16_bf16 tiles.  LDS holds two steps: one is
+// multiplied while the next is converted and written, and loads beyond it are
+// on their way in registers.
+//   [m][k] tiles lie in LDS as [rows][BK] with 16-byte columns swizzled by the
 //   row: the 16-byte fragment reads touch every bank once.
-//   [k][m] tiles lie as [BK][128] and are read by ds_read_b64_tr_b16, which
+//   [k][m] tiles lie as [BK][rows] and are read by ds_read_b64_tr_b16, which
 //   hands each lane 4 values down a column; 32-byte columns swizzled by k.
 // Sums are 32-bit in the accumulators.
+//
+// Bound by the matrix units: 46 to 62 percent busy in the long products (at
+// the clock such kernels run at, the library's bf16 product has 66), logits
+// 8192 x 50021 x 2048 bf16 in 1526 us, 1100 TFLOP/s; fp32 products of a few
+// hundred deep reach 150 to 170 TFLOP/s, about what the library's fp32 product
+// reaches at its best sizes.
 
 #include "token_ops.h"
 #include "token_device.h"
@@ -82,15 +89,9 @@ struct Params {
   float* picked;
   const float* lse;
   const float* ratio;     // [groups][n], null: all ones
+  float* rowsum;          // [groups][tiles_n * WN][m], may be null
   Scale scale;            // of what STORE writes
 };
-
-__device__ __forceinline__ float scale_of(const Scale& s, long long g) {
-  if (!s.num) return 1.f;
-  if (!s.den) return s.num[g];
-  // nothing counted: nothing to scale
-  return s.den[g] == 0.f ? 0.f : s.num[g] / s.den[g];
-}
 
 // Three bf16 parts of 8 floats, packed in pairs.
 __device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&o)[3]) {
@@ -340,6 +341,21 @@ __device__ __forceinline__ int acc_row(int r, int lane) {
   return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
 }
 
+// Of 2 * LEN values, lanes without bit `o` keep the sums of the first half,
+// lanes with it those of the second.
+template <int LEN, int N>
+__device__ __forceinline__ void fold(float (&sum)[N], int o, int lane,
+                                     int& lo) {
+  const bool up = lane & o;
+#pragma unroll
+  for (int i = 0; i < LEN; ++i) {
+    const float mine = up ? sum[LEN + i] : sum[i];
+    const float other = up ? sum[i] : sum[LEN + i];
+    sum[i] = mine + __shfl_xor(other, o, 64);
+  }
+  if (up) lo += LEN;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <Src S>
@@ -435,6 +451,11 @@ void gemm_kernel(Params p) {
       products(u, fa);
     }
   };
+  // Transposing reads, two to a fragment, are issued one unit ahead of their
+  // products (bf16 P'W 8192 x 2048 x 12544: 411 against 428 us, dY'X8 347
+  // against 377); plain ones are better left to the compiler, which needs the
+  // registers (logits 8192 x 50021 x 2048: 1526 against 1680 us).
+  constexpr bool AHEAD = KMA || KMB;
   constexpr int FIRST = MF;      // units that cover conversion and writing
 
   // Two tiles in LDS: one is multiplied while the next is converted and
@@ -450,7 +471,7 @@ void gemm_kernel(Params p) {
 #pragma unroll
     for (int u = 0; u < FIRST; ++u) read_a(sa[cur()], u, fa[u]);
     bf16x8 ahead[2][PA];
-    if (UNITS > FIRST) {
+    if (AHEAD && UNITS > FIRST) {
       read_b(sb[cur()], 1);
       read_a(sa[cur()], FIRST, ahead[FIRST & 1]);
     }
@@ -473,16 +494,21 @@ void gemm_kernel(Params p) {
     la.template load_whole<decltype(set)::value>();
     lb.template load_whole<decltype(set)::value>();
     __builtin_amdgcn_sched_barrier(0);
-    // fragments are read one unit ahead of their products
 #pragma unroll
     for (int u = FIRST; u < UNITS; ++u) {
-      if (u + 1 < UNITS) {
-        if ((u + 1) % MF == 0) read_b(sb[cur()], (u + 1) / MF);
-        read_a(sa[cur()], u + 1, ahead[(u + 1) & 1]);
+      if (AHEAD) {
+        if (u + 1 < UNITS) {
+          if ((u + 1) % MF == 0) read_b(sb[cur()], (u + 1) / MF);
+          read_a(sa[cur()], u + 1, ahead[(u + 1) & 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        products(u, ahead[u & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        if (u % MF == 0) read_b(sb[cur()], u / MF);
+        read_a(sa[cur()], u, ahead[0]);
+        products(u, ahead[0]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      products(u, ahead[u & 1]);
-      __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto checked_step = [&](int s, auto cur, auto set) {
@@ -661,6 +687,10 @@ void gemm_kernel(Params p) {
   }
 
   if constexpr (E == GRAD) {
+    // sums over this wave's tokens, 32 lanes still apart
+    float sum[MF * 16];
+#pragma unroll
+    for (int i = 0; i < MF * 16; ++i) sum[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const int n = n0 + j * 32 + (lane & 31);
@@ -686,34 +716,75 @@ void gemm_kernel(Params p) {
           float d = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e);
           if (mr + 4 * (lane >> 5) == row) d -= 1.f;
           d = live && m0 + mr + 4 * (lane >> 5) < M ? d * ratio : 0.f;
+          sum[i * 16 + r] += d;
           if (SA == F32)
             static_cast<float*>(p.out)[at + mr * p.out_ld] = d;
           else
             static_cast<bf16*>(p.out)[at + mr * p.out_ld] = (bf16)d;
         }
     }
+    if (p.rowsum) {
+      // Each exchange halves the values a lane answers for: after five, lane
+      // l holds the sums of values l * MF / 2 and on.
+      int lo = 0;
+      fold<MF * 8>(sum, 16, lane, lo);
+      fold<MF * 4>(sum, 8, lane, lo);
+      fold<MF * 2>(sum, 4, lane, lo);
+      fold<MF>(sum, 2, lane, lo);
+      fold<MF / 2>(sum, 1, lane, lo);
+      // one 32 x 32 tile a wave: 16 values, each still in a pair of lanes
+      if (MF == 1) sum[0] += __shfl_xor(sum[0], 1, 64);
+      constexpr int LEFT = MF / 2 > 0 ? MF / 2 : 1;
+      float* out = p.rowsum
+          + ((g * p.tiles_n + tn) * H::WN + wave % H::WN) * (long long)M;
+#pragma unroll
+      for (int i = 0; i < LEFT; ++i) {
+        const int v = lo + i;
+        const int m = m0 + v / 16 * 32 + acc_row(v % 16, lane);
+        if (m < M && (MF > 1 || !(lane & 1))) out[m] = sum[i];
+      }
+    }
   }
 }
 
-template <typename T>
+// out[g][i] = sum over splits of partial[split][g][i] (+ bias[i % n]), i over
+// the m * n outputs of a group; V values a thread.
+template <typename T, int V>
 __global__ __launch_bounds__(kThreads)
 void join_kernel(const float* __restrict__ partial, int splits,
-                 long long slab, long long m, long long n, T* out,
-                 long long out_ld, long long out_group, const T* bias,
-                 long long bias_group) {
-  const long long step = (long long)gridDim.x * kThreads;
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < slab;
-       i += step) {
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += partial[k * slab + i];
-    const long long c = i % n, row = i / n, g = row / m, r = row - g * m;
-    if (bias) s += to_f(bias[g * bias_group + c]);
-    out[g * out_group + r * out_ld + c] = from_f<T>(s);
+                 long long slab, long long size, long long n, T* out,
+                 long long out_group, const T* bias, long long bias_group) {
+  const long long g = blockIdx.y;
+  const long long step = (long long)gridDim.x * kThreads * V;
+  for (long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * V;
+       i < size; i += step) {
+    const float* p = partial + g * size + i;
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      float v[V];
+      load_n<V>(p + k * slab, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += v[j];
+    }
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        s[j] += to_f(bias[g * bias_group + (i + j) % n]);
+    }
+    T* o = out + g * out_group + i;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = from_f<T>(s[j]);
   }
 }
 
-// Merges the vocabulary tiles' (max, sum) of 32 tokens per block, 8 threads a
-// token, and leaves the block's loss sum and count in 64 bits.
+// Merges the vocabulary tiles' (max, sum) of R rows per block, 256 / R threads
+// a row, and leaves the block's loss sum and count in 64 bits.  Few rows are
+// given more threads each: a thread's tiles come one after another (7 rows,
+// 157 tiles: 3.8 us with R = 8 against 7.3 with 32).
+template <int R>
 __global__ __launch_bounds__(kThreads)
 void lse_kernel(const float2* __restrict__ part,
                 const float* __restrict__ picked,
@@ -721,15 +792,17 @@ void lse_kernel(const float2* __restrict__ part,
                 long long vocab, int tiles, long long rows,
                 float* __restrict__ lse, float* __restrict__ row_loss,
                 double2* __restrict__ sums) {
-  __shared__ float2 seg[8][32];
-  const int tl = threadIdx.x & 31, sl = threadIdx.x >> 5;
+  constexpr int SEGS = kThreads / R;
+  __shared__ float2 seg[SEGS][R];
+  const int tl = threadIdx.x % R, sl = threadIdx.x / R;
   const long long g = blockIdx.y;
-  for (long long blk = blockIdx.x; blk * 32 < rows; blk += gridDim.x) {
-    const long long n = blk * 32 + tl;
+  for (long long blk = blockIdx.x; blk * R < rows; blk += gridDim.x) {
+    const long long n = blk * R + tl;
     float mx = -INFINITY, sum = 0.f;
     if (n < rows) {
       const float2* q = part + g * tiles * rows + n;
-      for (int t = sl; t < tiles; t += 8) {
+#pragma unroll 4
+      for (int t = sl; t < tiles; t += SEGS) {
         const float2 v = q[(long long)t * rows];
         const float m = fmaxf(mx, v.x);
         const float ref = m == -INFINITY ? 0.f : m;
@@ -743,8 +816,7 @@ void lse_kernel(const float2* __restrict__ part,
     if (sl == 0) {
       double loss = 0.0, cnt = 0.0;
       if (n < rows) {
-#pragma unroll
-        for (int t = 1; t < 8; ++t) {
+        for (int t = 1; t < SEGS; ++t) {
           const float2 v = seg[t][tl];
           const float m = fmaxf(mx, v.x);
           const float ref = m == -INFINITY ? 0.f : m;
@@ -765,12 +837,12 @@ void lse_kernel(const float2* __restrict__ part,
         row_loss[g * rows + n] = row;
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        loss += __shfl_xor(loss, o, 32);
-        cnt += __shfl_xor(cnt, o, 32);
+      for (int o = R / 2; o > 0; o >>= 1) {
+        loss += __shfl_xor(loss, o, R);
+        cnt += __shfl_xor(cnt, o, R);
       }
       if (tl == 0 && sums)
-        sums[g * ((rows + 31) / 32) + blk] = make_double2(loss, cnt);
+        sums[g * ((rows + R - 1) / R) + blk] = make_double2(loss, cnt);
     }
     __syncthreads();
   }
@@ -822,30 +894,6 @@ void row_scale_kernel(const float* __restrict__ grad, long long rows,
   if (threadIdx.x == 0) top[g] = t;
   for (long long i = threadIdx.x; i < rows; i += kThreads)
     ratio[g * rows + i] = m == 0 ? 0.f : grad[g * rows + i] / t;
-}
-
-// A wave sums a row of the logits' gradient.
-template <typename T>
-__global__ __launch_bounds__(kThreads)
-void rowsum_kernel(const T* __restrict__ pt, long long ld, long long group,
-                   long long rows, long long cols, T* out,
-                   long long out_group, Scale scale) {
-  constexpr int V = Vec16<T>::n;
-  const int lane = threadIdx.x & 63;
-  const long long g = blockIdx.y;
-  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows;
-       r += (long long)gridDim.x * 4) {
-    const T* p = pt + g * group + r * ld;
-    float s = 0.f;
-    for (long long c = lane * V; c < cols; c += 64 * V) {
-      float v[V];
-      load_n<V>(p + c, v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s += v[j];
-    }
-    s = lanes_sum<64>(s);
-    if (lane == 0) out[g * out_group + r] = from_f<T>(s * scale_of(scale, g));
-  }
 }
 
 Op make_op(const Mat& m, bool kmajor, long long rows, long long k) {
@@ -982,19 +1030,23 @@ void gemm(const Gemm& g, hipStream_t s) {
 }
 
 void join_partials(const float* partial, int splits, long long groups,
-                   long long m, long long n, void* out, long long out_ld,
-                   long long out_group, const void* bias,
-                   long long bias_group, DType tout, hipStream_t s) {
-  const long long slab = groups * m * n;
-  const unsigned grid = grid_of(ceil_div(slab, kThreads));
-  if (tout == kF32)
-    join_kernel<float><<<grid, kThreads, 0, s>>>(
-        partial, splits, slab, m, n, static_cast<float*>(out), out_ld,
-        out_group, static_cast<const float*>(bias), bias_group);
-  else
-    join_kernel<bf16><<<grid, kThreads, 0, s>>>(
-        partial, splits, slab, m, n, static_cast<bf16*>(out), out_ld,
-        out_group, static_cast<const bf16*>(bias), bias_group);
+                   long long m, long long n, void* out, long long out_group,
+                   const void* bias, long long bias_group, DType tout,
+                   hipStream_t s) {
+  const long long size = m * n, slab = groups * size;
+  const bool four = size % 4 == 0;
+  const dim3 grid(grid_of(ceil_div(size, kThreads * (four ? 4 : 1))),
+                  (unsigned)groups);
+#define BLADES_JOIN(T, V)                                                  \
+  join_kernel<T, V><<<grid, kThreads, 0, s>>>(                             \
+      partial, splits, slab, size, n, static_cast<T*>(out), out_group,     \
+      static_cast<const T*>(bias), bias_group)
+  if (tout == kF32) {
+    if (four) BLADES_JOIN(float, 4); else BLADES_JOIN(float, 1);
+  } else {
+    if (four) BLADES_JOIN(bf16, 4); else BLADES_JOIN(bf16, 1);
+  }
+#undef BLADES_JOIN
 }
 
 static Size loss_size(const Loss& l) {
@@ -1005,7 +1057,15 @@ void loss_tile(const Loss& l, int* m, int* n) {
   *m = kTileM[loss_size(l)];
   *n = kTileN[loss_size(l)];
 }
-long long loss_sum_blocks(long long rows) { return ceil_div(rows, 32); }
+long long loss_row_parts(const Loss& l) {
+  const Size z = loss_size(l);
+  const int waves = z == LARGE ? Large::WN : z == SMALL ? Small::WN : Tiny::WN;
+  return ceil_div(l.rows, kTileN[z]) * waves;
+}
+static int lse_rows(long long rows) { return rows <= 4096 ? 8 : 32; }
+long long loss_sum_blocks(long long rows) {
+  return ceil_div(rows, lse_rows(rows));
+}
 
 namespace {
 Params loss_params(const Loss& l, long long v0, long long nv) {
@@ -1036,7 +1096,8 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
   if (l.t == kF32) launch<F32, false, F32, false, LSE>(p, l.groups, size, s);
   else launch<BF16, false, BF16, false, LSE>(p, l.groups, size, s);
   const long long blocks = loss_sum_blocks(l.rows);
-  lse_kernel<<<dim3(grid_of(blocks), (unsigned)l.groups), kThreads, 0, s>>>(
+  const auto merge = lse_rows(l.rows) == 8 ? lse_kernel<8> : lse_kernel<32>;
+  merge<<<dim3(grid_of(blocks), (unsigned)l.groups), kThreads, 0, s>>>(
       p.part, picked, l.target, l.ignore, l.vocab, p.tiles_m, l.rows, lse,
       row_loss, static_cast<double2*>(block_sums));
   if (loss)
@@ -1046,8 +1107,10 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
 
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
                      const float* lse, const float* ratio, void* pt,
-                     long long pt_ld, long long pt_group, hipStream_t s) {
+                     long long pt_ld, long long pt_group, float* rowsum,
+                     hipStream_t s) {
   Params p = loss_params(l, v0, nv);
+  p.rowsum = rowsum;
   p.lse = lse;
   p.ratio = ratio;
   p.out = pt;
@@ -1062,20 +1125,6 @@ void row_scale(const float* grad, long long groups, long long rows,
                float* top, float* ratio, hipStream_t s) {
   row_scale_kernel<<<dim3((unsigned)groups), kThreads, 0, s>>>(grad, rows,
                                                                top, ratio);
-}
-
-void rowsum(const void* pt, long long ld, long long group, long long groups,
-            long long rows, long long cols, void* out, long long out_group,
-            const Scale& scale, DType t, hipStream_t s) {
-  const dim3 grid(grid_of(ceil_div(rows, 4)), (unsigned)groups);
-  if (t == kF32)
-    rowsum_kernel<float><<<grid, kThreads, 0, s>>>(
-        static_cast<const float*>(pt), ld, group, rows, cols,
-        static_cast<float*>(out), out_group, scale);
-  else
-    rowsum_kernel<bf16><<<grid, kThreads, 0, s>>>(
-        static_cast<const bf16*>(pt), ld, group, rows, cols,
-        static_cast<bf16*>(out), out_group, scale);
 }
 
 }  // namespace token_ops

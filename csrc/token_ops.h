@@ -39,6 +39,18 @@ long long norm_partial_blocks(long long groups, long long rows, long long dim,
 void norm_forward(const NormArgs& a, DType t, hipStream_t s);
 void norm_backward(const NormArgs& a, DType t, hipStream_t s);
 
+// A factor per group: num[g], or num[g] / den[g] (0 where den is 0), or 1
+// where num is null.
+struct Scale {
+  const float* num;
+  const float* den;
+};
+
+// out[g][c] = scale[g] * sum over blocks of partial[g][block][c]
+void join_rows(const float* partial, long long groups, long long blocks,
+               long long cols, void* out, long long out_group,
+               const Scale& scale, DType t, hipStream_t s);
+
 // Sums over rows: out[g][c] = sum_r x[g][r][c], through a workspace of
 // groups * colsum_blocks() * cols floats.
 long long colsum_blocks(long long groups, long long rows, long long cols);
@@ -65,13 +77,6 @@ struct Mat {              // row-major, `ld` elements between rows
   bool padded;            // rows may be read, as zeros, up to `ld`
 };
 
-// A factor per group: num[g], or num[g] / den[g] (0 where den is 0), or 1
-// where num is null.
-struct Scale {
-  const float* num;
-  const float* den;
-};
-
 // out[g][m][n] = scale[g] * sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), 32-bit sums.
 //   a_kmajor: A is stored [k][m] instead of [m][k]; likewise b_kmajor.
 // With `partial` set and splits > 1 the contraction is cut into `splits`
@@ -95,11 +100,12 @@ struct Gemm {
 // Parts the contraction is best cut into (1: write `out` at once).
 int gemm_splits(const Gemm& g);
 void gemm(const Gemm& g, hipStream_t s);
-// out = sum over splits of partial (+ bias), rounded to tout
+// out = sum over splits of partial (+ bias), rounded to tout; a group's rows
+// lie without gaps
 void join_partials(const float* partial, int splits, long long groups,
-                   long long m, long long n, void* out, long long out_ld,
-                   long long out_group, const void* bias,
-                   long long bias_group, DType tout, hipStream_t s);
+                   long long m, long long n, void* out, long long out_group,
+                   const void* bias, long long bias_group, DType tout,
+                   hipStream_t s);
 
 // ----------------------------------------------- loss of a linear head
 struct Loss {
@@ -128,12 +134,12 @@ void row_scale(const float* grad, long long groups, long long rows,
 // onehot), token-minor, zero beyond rows and nv up to whole tiles.
 // The group's upstream factor stays out of it: rounded into the bf16 values
 // it would be one relative error, up to 2^-8, common to all of them.
+// rowsum (may be null): [groups][loss_row_parts()][nv] sums over rows, before
+// any rounding to bf16.
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
                      const float* lse, const float* ratio, void* pt,
-                     long long pt_ld, long long pt_group, hipStream_t s);
-// out[g][v] = scale * sum over the row of pt
-void rowsum(const void* pt, long long ld, long long group, long long groups,
-            long long rows, long long cols, void* out, long long out_group,
-            const Scale& scale, DType t, hipStream_t s);
+                     long long pt_ld, long long pt_group, float* rowsum,
+                     hipStream_t s);
+long long loss_row_parts(const Loss& l);
 
 }  // namespace token_ops
