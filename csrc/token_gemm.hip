@@ -365,7 +365,10 @@ __device__ __forceinline__ float bias_at(const void* p, long long i) {
 }
 
 template <Src SA, bool KMA, Src SB, bool KMB, typename H, Epi E>
-__global__ __launch_bounds__(H::THREADS)
+// Small fp32 blocks are held to 168 registers so that three share a compute
+// unit: 211 -> 196 us for the two gradient products of 16 x 500 x 5000 x 300.
+__global__ __launch_bounds__(H::THREADS,
+                             SrcOf<SA>::P == 3 && H::MF == 2 ? 3 : 1)
 void gemm_kernel(Params p) {
   constexpr int PA = SrcOf<SA>::P, PB = SrcOf<SB>::P;
   constexpr int MF = H::MF, NF = H::NF;
@@ -929,8 +932,8 @@ void launch(Params& p, long long groups, Size size, hipStream_t s) {
 }
 
 // Tile shape and parts of the contraction, by an estimate of the time.  A
-// compute unit works off blocks in rounds: one large, two small or three tiny
-// at once.  A round's time is its area and its depth plus a fixed part
+// compute unit works off blocks in rounds: one large, two small (three in
+// fp32) or three tiny at once.  A round's time is its area and its depth plus a fixed part
 // (filling the pipeline, the epilogue), which a large block alone does not
 // hide as well.  Measured: large tiles are 1.16 times as fast in the long run
 // (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
@@ -948,9 +951,12 @@ const int kTileN[3] = {Tiny::BN, Small::BN, Large::BN};
 // deep.  `products`: matrix instructions per multiplication (1, 3 or 6).
 Tiling tiling(long long groups, long long m, long long n, long long k,
               bool deep, int products) {
-  // rounds with up to 256 blocks (one a compute unit), and full ones
-  const int slots[3] = {768, 512, 256};
-  const double alone[3] = {0.5, 1.4, 4.0}, full[3] = {1.12, 2.32, 4.0};
+  // the time of a round by the blocks on a compute unit, 0 to 3
+  const bool parts = products > 1;
+  const int most_blocks[3] = {3, parts ? 3 : 2, 1};
+  const double round[3][4] = {{0, 0.5, 0.8, 1.12},
+                              {0, 1.5, 2.32, 3.25},
+                              {0, 4.0, 0, 0}};
   const double fixed[3] = {60, 50, 92};
   // 128 x 128 x 1 steps of a compute unit per microsecond
   const double rate = products == 6 ? 24 : products == 3 ? 45 : 135;
@@ -964,9 +970,9 @@ Tiling tiling(long long groups, long long m, long long n, long long k,
     // tiny tiles of a huge output: too many blocks, and never the best
     if (z == TINY && tiles > 1 << 16) continue;
     for (long long splits = 1; splits <= most; ++splits) {
-      const long long blocks = tiles * splits, rest = blocks % slots[z];
-      const double rounds = full[z] * (blocks / slots[z])
-          + (rest == 0 ? 0 : rest <= 256 ? alone[z] : full[z]);
+      const long long blocks = tiles * splits, slots = 256 * most_blocks[z];
+      const double rounds = round[z][most_blocks[z]] * (blocks / slots)
+          + round[z][ceil_div(blocks % slots, 256)];
       double us = rounds * (ceil_div(k, splits) + fixed[z]) / rate;
       // the parts are written, read and joined
       if (splits > 1) us += 4 + (2 * splits + 1) * 4e-6 * m * n * groups / 4;
