@@ -304,7 +304,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     """Cross entropy of the logits ``x @ weight.T + bias`` with ``target``,
     in float32, computed in tiles: the [rows, vocab] logits are never stored.
     The backward pass computes them again, a piece of the vocabulary at a
-    time (at most 256 MiB of their gradient exists at once, or 512 words).
+    time (at most 256 MiB of their gradient exists at once, or 512 words); it
+    takes fewer than 2**22 rows a client.
 
     ``x``: [..., dim]; ``weight``: [vocab, dim]; ``bias``: [vocab] or None;
     ``target``: int64, x's leading shape.  Rows whose target is
