@@ -10,8 +10,8 @@
 float32 and bfloat16.  GPU tensors run the HIP kernels of ``csrc/`` (and
 refuse to run without them) through dispatcher ops of the extension; CPU
 tensors run the plain forms of :mod:`torch_ref` under the autograd functions
-below, which have the same rules.  Every operator runs under ``torch.func.grad`` and
-``torch.func.vmap`` in either nesting: a vmapped call is ONE launch over all
+below, which have the same rules.  Every operator runs under
+``torch.func.grad`` and ``torch.func.vmap`` in either nesting: a vmapped call is ONE launch over all
 clients ("groups" below), with shared or per-client parameters, and
 ``vmap(grad(...))`` gets the parameters' gradients per client from the
 kernels.  A vmap inside a vmap whose parameters or gradients are per client at

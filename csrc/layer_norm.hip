@@ -14,7 +14,8 @@
 // repeat bit for bit.  Rows wider than the registers hold (or wide rows
 // without 16-byte alignment) take kernels that read the row again instead.
 // Measured: 16383 x 4096 bf16 forward 63 us (4.3 TB/s), backward 100 us
-// (4.0 TB/s, 11 us more to join); 204800 x 128 fp32 in 100 clients 37 and 61 us.
+// (4.0 TB/s, 11 us more to join); 204800 x 128 fp32 in 100 clients 37 and
+// 61 us.
 
 #include "token_ops.h"
 #include "token_device.h"

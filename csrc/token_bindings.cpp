@@ -1142,8 +1142,9 @@ Int3 linear_grad_vmap(const Tensor& dy, const Tensor& w, const Tensor& q,
     return linear_grad_op().call(dy, w, q, e, groups, wx, ww, wb);
   refuse_nested(groups, "linear_act8");
   return v.close(
-      linear_grad_op().call(v.all(dy), v.param(w), ww ? v.all(q) : q,
-                            ww ? v.all(e) : e, v.size, wx, ww, wb),
+      linear_grad_op().call(v.all(dy), v.param(w),
+                            ww ? v.all(q) : v.param(q),
+                            ww ? v.all(e) : v.param(e), v.size, wx, ww, wb),
       wx, ww, wb);
 }
 

@@ -46,7 +46,10 @@ enum Size { TINY, SMALL, LARGE };
 template <Src S> struct SrcOf;
 template <> struct SrcOf<F32> { using T = float; static constexpr int P = 3; };
 template <> struct SrcOf<BF16> { using T = bf16; static constexpr int P = 1; };
-template <> struct SrcOf<ACT8> { using T = int8_t; static constexpr int P = 1; };
+template <> struct SrcOf<ACT8> {
+  using T = int8_t;
+  static constexpr int P = 1;
+};
 
 // Waves of a block along m and n, each wave's 32 x 32 tiles, and the depth of
 // a step for one-part and for three-part operands.
@@ -877,16 +880,18 @@ void loss_sum_kernel(const double2* __restrict__ sums, long long blocks,
   }
 }
 
-// The largest magnitude of a group's upstream row gradients, and the rows'
-// ratios to it.
+// The largest finite magnitude of a group's upstream row gradients, and the
+// rows' ratios to it; a row's that is not finite stays its own matter.
 __global__ __launch_bounds__(kThreads)
 void row_scale_kernel(const float* __restrict__ grad, long long rows,
                       float* __restrict__ top, float* __restrict__ ratio) {
   __shared__ uint32_t red[4];
   const long long g = blockIdx.x;
-  uint32_t m = 0;                      // bit patterns order NaN above all
-  for (long long i = threadIdx.x; i < rows; i += kThreads)
-    m = max(m, __float_as_uint(grad[g * rows + i]) & 0x7fffffffu);
+  uint32_t m = 0;                      // bit patterns order as magnitudes do
+  for (long long i = threadIdx.x; i < rows; i += kThreads) {
+    const uint32_t b = __float_as_uint(grad[g * rows + i]) & 0x7fffffffu;
+    if (b < 0x7f800000u) m = max(m, b);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
     m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
@@ -895,8 +900,11 @@ void row_scale_kernel(const float* __restrict__ grad, long long rows,
   m = max(max(red[0], red[1]), max(red[2], red[3]));
   const float t = __uint_as_float(m);
   if (threadIdx.x == 0) top[g] = t;
-  for (long long i = threadIdx.x; i < rows; i += kThreads)
-    ratio[g * rows + i] = m == 0 ? 0.f : grad[g * rows + i] / t;
+  for (long long i = threadIdx.x; i < rows; i += kThreads) {
+    const float v = grad[g * rows + i];
+    const bool finite = (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u;
+    ratio[g * rows + i] = !finite ? v : m == 0 ? 0.f : v / t;
+  }
 }
 
 Op make_op(const Mat& m, bool kmajor, long long rows, long long k) {
@@ -933,9 +941,9 @@ void launch(Params& p, long long groups, Size size, hipStream_t s) {
 
 // Tile shape and parts of the contraction, by an estimate of the time.  A
 // compute unit works off blocks in rounds: one large, two small (three in
-// fp32) or three tiny at once.  A round's time is its area and its depth plus a fixed part
-// (filling the pipeline, the epilogue), which a large block alone does not
-// hide as well.  Measured: large tiles are 1.16 times as fast in the long run
+// fp32) or three tiny at once.  A round's time is its area and its depth plus
+// a fixed part (filling the pipeline, the epilogue), which a large block alone
+// does not hide as well.  Measured: large tiles are 1.16 times as fast in the long run
 // (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
 // contractions (fp32 16 x 500 x 5000 x 300: 171 against 197 us), tiny ones
 // where few blocks would leave units idle (fp32 2048 x 128 x 128: 8.7 against

@@ -77,7 +77,8 @@ struct Mat {              // row-major, `ld` elements between rows
   bool padded;            // rows may be read, as zeros, up to `ld`
 };
 
-// out[g][m][n] = scale[g] * sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), 32-bit sums.
+// out[g][m][n] = scale[g] * sum_k A[g](m,k) * B[g](n,k) (+ bias[g][n]), sums in
+// 32 bits.
 //   a_kmajor: A is stored [k][m] instead of [m][k]; likewise b_kmajor.
 // With `partial` set and splits > 1 the contraction is cut into `splits`
 // parts whose sums go to partial[split][g][m][n] and are joined afterwards;
@@ -119,8 +120,8 @@ struct Loss {
 };
 // Tiles the loss is computed in: m words by n rows.
 void loss_tile(const Loss& l, int* m, int* n);
-// part: [groups][vocabulary tiles][rows] float2; picked: [groups][rows] float.  Writes
-// lse and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
+// part: [groups][vocabulary tiles][rows] float2; picked: [groups][rows] float.
+// Writes lse and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
 // group and the number of counted rows, through block_sums
 // [groups][loss_sum_blocks(rows)] double2.
 long long loss_sum_blocks(long long rows);

@@ -420,6 +420,23 @@ def test_loss_target_outside_the_vocabulary(device, bad):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_loss_non_finite_upstream_row(device, bad):
+    """Only the row's own input gradient, and the parameters', are lost."""
+    x, w, y, b = loss_inputs(6, 16, 50, torch.float32, device)
+    x.requires_grad_(), w.requires_grad_()
+    rows = ops.linear_cross_entropy(x, w, y, b, reduction="none")
+    up = torch.ones_like(rows)
+    want, = torch.autograd.grad(rows, x, up, retain_graph=True)
+    up[4] = bad
+    up[5] = 0
+    dx, dw = torch.autograd.grad(rows, (x, w), up)
+    assert not dx[4].isfinite().any() and not dw.isfinite().any()
+    assert torch.equal(dx[5], torch.zeros_like(dx[5]))
+    near(dx[:4], want[:4], 1e-6 * want[:4].abs() + 1e-7)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_loss_ignore_index_in_the_vocabulary(device):
     x, w, y, b = loss_inputs(12, 16, 50, torch.float32, device)
     y[1] = 3
@@ -812,6 +829,22 @@ def test_vmap_loss_rows(device):
         want.append(torch.autograd.grad(f(leaf, y[i]).square().sum(),
                                         leaf)[0])
     close(g(x, y), torch.stack(want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+def test_only_the_input_needs_a_gradient_of_tracked_parameters(device, fn):
+    """vmap(grad) in the input alone while outer levels track parameters."""
+    w, b, x, y, up = population(fn, 3, device)
+    f = fn
+    w0, b0 = w[0].clone().requires_grad_(), b[0].clone().requires_grad_()
+
+    def in_x(x, y, up):
+        out, pull = torch.func.vjp(lambda x: f(w0, b0, x, y), x)
+        return pull(up)[0]
+    got = torch.func.vmap(in_x)(x, y, up)
+    want = one_by_one(f, w[:1].expand_as(w), b[:1].expand_as(b), x, y, up)[3]
+    close(got.detach(), want)
 
 
 @pytest.mark.parametrize("device", DEVICES)
