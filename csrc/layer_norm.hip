@@ -13,9 +13,9 @@
 // each, summed in a fixed order by a second kernel: no atomics, so results
 // repeat bit for bit.  Rows wider than the registers hold (or wide rows
 // without 16-byte alignment) take kernels that read the row again instead.
-// Measured: 16383 x 4096 bf16 forward 63 us (4.3 TB/s), backward 100 us
-// (4.0 TB/s, 11 us more to join); 204800 x 128 fp32 in 100 clients 37 and
-// 61 us.
+// Measured: 16383 x 4096 bf16 forward 62 us (4.3 TB/s), backward 82 us
+// (4.9 TB/s, 7 us more to join); 204800 x 128 fp32 in 100 clients 37 and
+// 59 us.
 
 #include "token_ops.h"
 #include "token_device.h"
@@ -28,7 +28,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // Sum over the TPR threads of a row.  For TPR == 256 `red` holds one slot per
-// wave and value; the trailing barrier lets the next call reuse it.
+// wave and value.  There is one barrier, between writing and reading it: calls
+// take turns with two such arrays, so that the other one's barrier lies
+// between reading an array and writing it again.
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
   constexpr int W = TPR < 64 ? TPR : 64;
@@ -48,7 +50,41 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
       for (int w = 0; w < TPR / 64; ++w) s += red[w * N + i];
       v[i] = s;
     }
-    __syncthreads();
+  }
+}
+
+// VEC values as they lie in memory
+template <typename T, int VEC> struct Packed { T v[VEC]; };
+template <> struct Packed<float, 4> { f32x4 v; };
+template <> struct Packed<bf16, 8> { u32x4 v; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void fetch(const T* p, Packed<T, VEC>& r) {
+  if constexpr (VEC == Vec16<T>::n) {
+    r.v = *reinterpret_cast<const decltype(r.v)*>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) r.v[j] = p[j];
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void unpack(const Packed<float, VEC>& r,
+                                       float (&v)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[j] = r.v[j];
+}
+template <int VEC>
+__device__ __forceinline__ void unpack(const Packed<bf16, VEC>& r,
+                                       float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(r.v[j] << 16);
+      v[2 * j + 1] = __uint_as_float(r.v[j] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)r.v[j];
   }
 }
 
@@ -56,7 +92,7 @@ template <typename T, int VEC, int NV, int TPR>
 __global__ __launch_bounds__(kThreads)
 void norm_fwd_kernel(NormArgs a) {
   constexpr int RPB = kThreads / TPR;
-  __shared__ float red[8];
+  __shared__ float red[2][8];
   const int lane = threadIdx.x % TPR;
   const long long total = a.groups * a.rows;
   const int dim = (int)a.dim;
@@ -81,7 +117,7 @@ void norm_fwd_kernel(NormArgs a) {
       for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
     }
     float one[1] = {s[0]};
-    row_sum<TPR, 1>(one, red);
+    row_sum<TPR, 1>(one, red[0]);
     const float inv = 1.f / (float)dim;
     float mean = one[0] * inv;
     // The centred values' own mean corrects what the first sum rounded away,
@@ -99,7 +135,7 @@ void norm_fwd_kernel(NormArgs a) {
         }
       }
     }
-    row_sum<TPR, 2>(s, red);
+    row_sum<TPR, 2>(s, red[1]);
     const float off = s[0] * inv;
     const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
     mean += off;
@@ -137,7 +173,7 @@ __global__ __launch_bounds__(kThreads)
 void norm_bwd_kernel(NormArgs a) {
   constexpr int RPB = kThreads / TPR;
   constexpr int SPAN = TPR * VEC * NV;            // columns a row slot holds
-  __shared__ float red[8];
+  __shared__ float red[2][8];
   __shared__ float comb[PARAMS && TPR <= 64 ? 4 * SPAN : 1];
   const int lane = threadIdx.x % TPR;
   const int dim = (int)a.dim;
@@ -163,27 +199,46 @@ void norm_bwd_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
 
+  // The next row's values are fetched while this one's are reduced, where
+  // registers allow (16383 x 4096 bf16: 82 us against 99; the forward pass,
+  // whose blocks are many and short, gains nothing from it: 65 against 62).
+  constexpr bool AHEAD = NV * VEC <= 32;
   const long long step = (long long)gridDim.x * RPB;
-  for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += step) {
+  Packed<T, VEC> px[NV], pd[NV];
+  float pm = 0.f, pr = 0.f;
+  auto fetch_row = [&](long long r0) {
+    const long long r = r0 + threadIdx.x / TPR;
+    if (r < a.rows) {                             // uniform over a row slot
+      const long long row = base + r;
+      pm = a.mean[row];
+      pr = a.rstd[row];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * VEC;
+        if (c < dim) {
+          fetch<T, VEC>(static_cast<const T*>(a.x) + row * a.dim + c, px[i]);
+          fetch<T, VEC>(static_cast<const T*>(a.dy) + row * a.dim + c, pd[i]);
+        }
+      }
+    }
+  };
+  int turn = 0;
+  if (AHEAD) fetch_row((long long)blockIdx.x * RPB);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows;
+       r0 += step, turn ^= 1) {
     const long long r = r0 + threadIdx.x / TPR;
     const bool live = r < a.rows;                 // uniform over a row slot
     const long long row = base + (live ? r : 0);
-    const T* x = static_cast<const T*>(a.x) + row * a.dim;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dim;
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    if (!AHEAD) fetch_row(r0);
+    const float mean = pm, rstd = pr;
     float h[NV][VEC], d[NV][VEC];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (live && c < dim) {
-        load_n<VEC>(x + c, h[i]);
-        load_n<VEC>(dy + c, d[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { h[i][j] = mean; d[i][j] = 0.f; }
-      }
+      unpack(px[i], h[i]);
+      unpack(pd[i], d[i]);
     }
+    if (AHEAD) fetch_row(r0 + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
@@ -201,7 +256,7 @@ void norm_bwd_kernel(NormArgs a) {
         }
       }
     }
-    row_sum<TPR, 2>(s, red);
+    row_sum<TPR, 2>(s, red[turn]);
     const float c1 = s[0] * inv, c2 = s[1] * inv;
     T* dx = static_cast<T*>(a.y) + row * a.dim;
 #pragma unroll
@@ -261,7 +316,7 @@ void norm_bwd_kernel(NormArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads)
 void norm_fwd_wide_kernel(NormArgs a) {
-  __shared__ float red[8];
+  __shared__ float red[2][8];
   for (long long row = blockIdx.x; row < a.groups * a.rows;
        row += gridDim.x) {
     const long long g = row / a.rows;
@@ -270,7 +325,7 @@ void norm_fwd_wide_kernel(NormArgs a) {
     float one[1] = {0.f};
     for (long long c = threadIdx.x; c < a.dim; c += kThreads)
       one[0] += to_f(x[c]);
-    row_sum<256, 1>(one, red);
+    row_sum<256, 1>(one, red[0]);
     float mean = one[0] * inv;
     float s[2] = {0.f, 0.f};
     for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
@@ -278,7 +333,7 @@ void norm_fwd_wide_kernel(NormArgs a) {
       s[0] += d;
       s[1] += d * d;
     }
-    row_sum<256, 2>(s, red);
+    row_sum<256, 2>(s, red[1]);
     const float off = s[0] * inv;
     const float rstd = 1.f / sqrtf(fmaxf(s[1] * inv - off * off, 0.f) + a.eps);
     mean += off;
@@ -298,9 +353,10 @@ void norm_fwd_wide_kernel(NormArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads)
 void norm_bwd_wide_kernel(NormArgs a) {
-  __shared__ float red[8];
+  __shared__ float red[2][8];
+  int turn = 0;
   for (long long row = blockIdx.x; row < a.groups * a.rows;
-       row += gridDim.x) {
+       row += gridDim.x, turn ^= 1) {
     const long long g = row / a.rows;
     const T* x = static_cast<const T*>(a.x) + row * a.dim;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dim;
@@ -314,7 +370,7 @@ void norm_bwd_wide_kernel(NormArgs a) {
       s[0] += d;
       s[1] += d * h;
     }
-    row_sum<256, 2>(s, red);
+    row_sum<256, 2>(s, red[turn]);
     const float inv = 1.f / (float)a.dim;
     const float c1 = s[0] * inv, c2 = s[1] * inv;
     for (long long c = threadIdx.x; c < a.dim; c += kThreads) {
@@ -532,13 +588,16 @@ void backward_t(const NormArgs& a, hipStream_t s) {
 }  // namespace
 
 // Blocks per group of the backward kernel.  About 1024 in all (4 per compute
-// unit) keep the chip full; more only add partial rows to join.
+// unit) keep the chip full; blocks that own a whole wide row are as fast with
+// 512, and leave half the partial rows to join (16383 x 4096 bf16: 82 + 7 us
+// against 94 + 11).
 long long norm_partial_blocks(long long groups, long long rows, long long dim,
                               DType t) {
   const int vec = t == kF32 ? 4 : 8;
   const int shape = norm_shape(ceil_div(dim, dim % vec ? 1 : vec));
   const long long rpb = shape < 0 ? 1 : kThreads / kTpr[shape];
-  const long long want = std::max<long long>(1, ceil_div(1024, groups));
+  const long long want =
+      std::max<long long>(1, ceil_div(rpb == 1 ? 512 : 1024, groups));
   return std::max<long long>(1, std::min(want, ceil_div(rows, rpb)));
 }
 
