@@ -121,6 +121,21 @@ typedef f32x4 f32x4_u __attribute__((aligned(4)));
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 typedef u32x2 u32x2_u __attribute__((aligned(1)));
 
+template <typename T>
+using Global = const __attribute__((address_space(1))) T*;
+
+// A pointer that is the same for all threads, held in scalar registers: left
+// to itself the compiler adds each thread's offset to it once and keeps the
+// sums, two registers a chunk, and spills (8-bit weight gradient 32768 x 4096
+// x 1024: 356 us so, 320 with the offsets alone; other products 1 to 4 %).
+template <typename T>
+__device__ __forceinline__ Global<T> scalar(Global<T> p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return reinterpret_cast<Global<T>>((uint64_t)hi << 32 | lo);
+}
+
 template <Src S> struct Raw { u32x4 v; };
 template <> struct Raw<F32> { f32x4 x, y; };
 template <> struct Raw<ACT8> { u32x2 v; uint32_t e; };
@@ -134,8 +149,8 @@ struct Loader {
   static constexpr int N = ROWS * BK / 8 / THREADS;     // chunks a thread
   static constexpr int PLANE = ROWS * BK;               // bf16 values
   static_assert(N >= 1 && N * 8 * THREADS == ROWS * BK);
-  const char* base;      // the next step's tile, the same for all threads
-  const uint8_t* ebase;
+  Global<char> base;     // the next step's tile, the same for all threads
+  Global<uint8_t> ebase;
   uint32_t off[N], eoff[N];                // bytes from there to a chunk
   long long ld, e_ld;
   int ext, left[N];      // [k][m]: end of a row, values from a chunk to it
@@ -151,10 +166,10 @@ struct Loader {
     kend = kend_;
     krows = krows_;
     const int row0 = tile * ROWS;
-    base = static_cast<const char*>(o.p)
+    base = (Global<char>)o.p
         + (g * o.group + (KM ? k0 * ld + row0 : row0 * ld + k0)) * sizeof(T);
     if constexpr (S == ACT8)
-      ebase = o.e + g * o.e_group + k0 * e_ld + (row0 >> 7);
+      ebase = (Global<uint8_t>)o.e + g * o.e_group + k0 * e_ld + (row0 >> 7);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = i * THREADS + threadIdx.x;
@@ -177,12 +192,13 @@ struct Loader {
     }
   }
 
-  __device__ __forceinline__ const T* at(int i) const {
-    return reinterpret_cast<const T*>(base + off[i]);
+  __device__ __forceinline__ Global<T> at(int i) const {
+    return reinterpret_cast<Global<T>>(base + off[i]);
   }
   __device__ __forceinline__ void advance() {
     base += (KM ? BK * ld : (long long)BK) * (long long)sizeof(T);
-    if constexpr (S == ACT8) ebase += BK * e_ld;
+    base = scalar(base);
+    if constexpr (S == ACT8) ebase = scalar(ebase + BK * e_ld);
   }
 
   // Whether the step from k0 can be read as it lies.  A [k][m] row's last
@@ -197,13 +213,15 @@ struct Loader {
     Raw<S>(&raw)[N] = raws[SET];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      // 32 bits here, widened by the load itself
+      asm("" : "+v"(off[i]));
       if constexpr (S == F32) {
-        raw[i].x = *reinterpret_cast<const f32x4_u*>(at(i));
-        raw[i].y = *reinterpret_cast<const f32x4_u*>(at(i) + 4);
+        raw[i].x = *reinterpret_cast<Global<f32x4_u>>(at(i));
+        raw[i].y = *reinterpret_cast<Global<f32x4_u>>(at(i) + 4);
       } else if constexpr (S == BF16) {
-        raw[i].v = *reinterpret_cast<const u32x4_u*>(at(i));
+        raw[i].v = *reinterpret_cast<Global<u32x4_u>>(at(i));
       } else {
-        raw[i].v = *reinterpret_cast<const u32x2_u*>(at(i));
+        raw[i].v = *reinterpret_cast<Global<u32x2_u>>(at(i));
         raw[i].e = ebase[eoff[i]];
       }
     }
@@ -233,13 +251,13 @@ struct Loader {
           raw[i].y[j] = 4 + j < valid ? at(i)[4 + j] : 0.f;
         }
       } else if constexpr (S == BF16) {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(at(i));
+        const Global<uint16_t> h = reinterpret_cast<Global<uint16_t>>(at(i));
         raw[i].v = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (j < valid) raw[i].v[j >> 1] |= (uint32_t)h[j] << (16 * (j & 1));
       } else {
-        const uint8_t* h = reinterpret_cast<const uint8_t*>(at(i));
+        const Global<uint8_t> h = reinterpret_cast<Global<uint8_t>>(at(i));
         raw[i].v = u32x2{0, 0};
         raw[i].e = valid > 0 ? ebase[eoff[i]] : 0;
 #pragma unroll
