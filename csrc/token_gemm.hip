@@ -961,11 +961,11 @@ void launch(Params& p, long long groups, Size size, hipStream_t s) {
 // compute unit works off blocks in rounds: one large, two small (three in
 // fp32) or three tiny at once.  A round's time is its area and its depth plus
 // a fixed part (filling the pipeline, the epilogue), which a large block alone
-// does not hide as well.  Measured: large tiles are 1.16 times as fast in the long run
-// (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on short
-// contractions (fp32 16 x 500 x 5000 x 300: 171 against 197 us), tiny ones
-// where few blocks would leave units idle (fp32 2048 x 128 x 128: 8.7 against
-// 19.7 us).
+// does not hide as well.  Measured: large tiles are 1.16 times as fast in the
+// long run (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on
+// short contractions (fp32 16 x 500 x 5000 x 300: 170 against 187 us), tiny
+// ones where few blocks would leave units idle (fp32 2048 x 128 x 128: 8.7
+// against 19.7 us).
 struct Tiling {
   Size size;
   int splits;
