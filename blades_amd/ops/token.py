@@ -350,42 +350,44 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
 
 class _GeluGrad(_NoSecond):
     @staticmethod
-    def forward(dy, q, e):
+    def forward(dy, q, e, tie):
         return _ref.gelu_backward(dy.contiguous(), q.contiguous(),
-                                          e.contiguous())
+                                  e.contiguous())
 
     @staticmethod
     def setup_context(ctx, inputs, output):
         pass
 
     @staticmethod
-    def vmap(info, in_dims, dy, q, e):
+    def vmap(info, in_dims, dy, q, e, tie):
         n = info.batch_size
         return _GeluGrad.apply(*(_batched(t, d, n) for t, d in
-                                 zip((dy, q, e), in_dims))), 0
+                                 zip((dy, q, e), in_dims)), tie), 0
 
 
 class _Gelu8(Function):
+    # The 8-bit values carry no history; `tie`, empty, does, so that their
+    # gradient function sees that it depends on x.
+
     @staticmethod
     def forward(x, keep):
-        return tuple(_ref.gelu_forward(x.contiguous(), keep))
+        return (*_ref.gelu_forward(x.contiguous(), keep), x.new_empty(0))
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        _, q, e = output
+        _, q, e, tie = output
         ctx.mark_non_differentiable(q, e)
-        ctx.save_for_backward(q, e)
+        ctx.save_for_backward(q, e, tie)
 
     @staticmethod
-    def backward(ctx, dy, _q, _e):
-        q, e = ctx.saved_tensors
-        return _GeluGrad.apply(dy, q, e), None
+    def backward(ctx, dy, _q, _e, _tie):
+        return _GeluGrad.apply(dy, *ctx.saved_tensors), None
 
     @staticmethod
     def vmap(info, in_dims, x, keep):
         per = 0 if keep else None
         return (_Gelu8.apply(_batched(x, in_dims[0], info.batch_size), keep),
-                (0, per, per))
+                (0, per, per, None))
 
 
 def gelu_act8(x: Tensor) -> Tensor:
@@ -428,7 +430,7 @@ def _product(x: Tensor, w: Tensor, groups: int, transpose: bool, b=None):
 
 class _LinearGrad(_NoSecond):
     @staticmethod
-    def forward(dy, w, q, e, groups, wants):
+    def forward(dy, w, q, e, tie, groups, wants):
         g = max(groups, 1)
         dx = (_product(dy, w, groups, False) if wants[0]
               else dy.new_empty(0))
@@ -451,18 +453,19 @@ class _LinearGrad(_NoSecond):
         pass
 
     @staticmethod
-    def vmap(info, in_dims, dy, w, q, e, groups, wants):
+    def vmap(info, in_dims, dy, w, q, e, tie, groups, wants):
         _refuse_nested(groups, "linear_act8")
         n = info.batch_size
         q, e = ((_batched(q, in_dims[2], n), _batched(e, in_dims[3], n))
                 if wants[1] else (q, e))
         out = _LinearGrad.apply(_batched(dy, in_dims[0], n),
-                                _param_batched(w, in_dims[1]), q, e, n, wants)
+                                _param_batched(w, in_dims[1]), q, e, tie, n,
+                                wants)
         return out, tuple(0 if want else None for want in wants)
 
 
 class _Linear8(Function):
-    # groups: as for _Norm
+    # groups: as for _Norm; tie: as for _Gelu8
 
     @staticmethod
     def forward(x, w, b, keep, groups):
@@ -472,23 +475,25 @@ class _Linear8(Function):
         else:
             q = e = x.new_empty(0, dtype=torch.uint8)
             e = e.clone()
-        return y, q, e
+        return y, q, e, x.new_empty(0)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
         _, w, b, _, groups = inputs
-        _, q, e = output
+        _, q, e, tie = output
         ctx.mark_non_differentiable(q, e)
-        ctx.save_for_backward(w, q, e)
+        ctx.save_for_backward(w, q, e, tie)
         ctx.groups = groups
         ctx.has_b = b is not None
 
     @staticmethod
-    def backward(ctx, dy, _q, _e):
-        w, q, e = ctx.saved_tensors
+    def backward(ctx, dy, _q, _e, _tie):
+        w, q, e, tie = ctx.saved_tensors
         wants = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                  ctx.has_b and ctx.needs_input_grad[2])
-        dx, dw, db = _LinearGrad.apply(dy, w, q, e, ctx.groups, wants)
+        # only the weight's gradient depends on the layer's input
+        dx, dw, db = _LinearGrad.apply(dy, w, q, e, tie if wants[1] else None,
+                                       ctx.groups, wants)
         return (dx if wants[0] else None, dw if wants[1] else None,
                 db if wants[2] else None, None, None)
 
@@ -501,7 +506,7 @@ class _Linear8(Function):
             w, b, groups = (_batched(w, in_dims[1], n),
                             _batched(b, in_dims[2], n), n)
         per = 0 if keep else None
-        return _Linear8.apply(x, w, b, keep, groups), (0, per, per)
+        return _Linear8.apply(x, w, b, keep, groups), (0, per, per, None)
 
 
 def linear_act8(x: Tensor, weight: Tensor,

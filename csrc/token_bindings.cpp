@@ -590,22 +590,30 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
 // `groups`: 0, or the number of clients on the leading axis of the inputs.
 // A gradient op called with groups gives the parameters' gradients per
 // client.
+//
+// The 8-bit input that GELU and linear layers keep is integers and carries no
+// autograd history.  An empty float tensor, `tie`, goes with it: it has a
+// history at every level that tracks the input, so that the gradient ops see
+// that their result depends on it.
 
 using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using Int3 = std::tuple<Tensor, Tensor, Tensor>;
+using Int4 = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 
 using NormSig = Int3(const Tensor&, const OptTensor&, const OptTensor&, double,
                      int64_t);
 using NormGradSig = Int3(const Tensor&, const Tensor&, const OptTensor&,
                          const Tensor&, const Tensor&, int64_t, bool);
-using GeluSig = Int3(const Tensor&, bool);
-using GeluGradSig = Tensor(const Tensor&, const Tensor&, const Tensor&);
-using LinearSig = Int3(const Tensor&, const Tensor&, const OptTensor&, bool,
+using GeluSig = Int4(const Tensor&, bool);
+using GeluGradSig = Tensor(const Tensor&, const Tensor&, const Tensor&,
+                           const Tensor&);
+using LinearSig = Int4(const Tensor&, const Tensor&, const OptTensor&, bool,
                        int64_t);
 using LinearGradSig = Int3(const Tensor&, const Tensor&, const Tensor&,
-                           const Tensor&, int64_t, bool, bool, bool);
+                           const Tensor&, const Tensor&, int64_t, bool, bool,
+                           bool);
 using LossSig = Int3(const Tensor&, const Tensor&, const Tensor&,
                      const OptTensor&, int64_t, int64_t, int64_t);
 using LossGradSig = Int3(const Tensor&, const Tensor&, const Tensor&,
@@ -673,10 +681,12 @@ Int3 norm_grad_cuda(const Tensor& dy, const Tensor& x, const OptTensor& w,
           ungroup(db, groups, params)};
 }
 
-Int3 gelu_cuda(const Tensor& x, bool keep) {
-  return gelu_forward_t(x.contiguous(), keep);
+Int4 gelu_cuda(const Tensor& x, bool keep) {
+  return std::tuple_cat(gelu_forward_t(x.contiguous(), keep),
+                        std::make_tuple(at::empty({0}, x.options())));
 }
-Tensor gelu_grad_cuda(const Tensor& dy, const Tensor& q, const Tensor& e) {
+Tensor gelu_grad_cuda(const Tensor& dy, const Tensor& q, const Tensor& e,
+                      const Tensor&) {
   return gelu_backward_t(dy.contiguous(), q.contiguous(), e.contiguous());
 }
 
@@ -686,7 +696,7 @@ bool plain_product(const Tensor& x, const Tensor& w) {
   return w.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.numel() > 0;
 }
 
-Int3 linear_cuda(const Tensor& x, const Tensor& w, const OptTensor& b,
+Int4 linear_cuda(const Tensor& x, const Tensor& w, const OptTensor& b,
                  bool keep, int64_t groups) {
   c10::DeviceGuard guard(x.device());
   Tensor y;
@@ -705,12 +715,12 @@ Int3 linear_cuda(const Tensor& x, const Tensor& w, const OptTensor& b,
     q = at::empty({0}, x.options().dtype(at::kChar));
     e = at::empty({0}, x.options().dtype(at::kByte));
   }
-  return {y.view(shape), q, e};
+  return {y.view(shape), q, e, at::empty({0}, x.options())};
 }
 
 Int3 linear_grad_cuda(const Tensor& dy, const Tensor& w, const Tensor& q,
-                      const Tensor& e, int64_t groups, bool want_x,
-                      bool want_w, bool want_b) {
+                      const Tensor& e, const Tensor&, int64_t groups,
+                      bool want_x, bool want_w, bool want_b) {
   c10::DeviceGuard guard(dy.device());
   const Tensor dy3 = groups3(dy, groups);
   Tensor dx, dw, db;
@@ -794,16 +804,16 @@ struct NormNode : public TokenNode {            // x, w, mean, rstd
   }
 };
 
-struct GeluNode : public TokenNode {            // q, e
+struct GeluNode : public TokenNode {            // q, e, tie
   std::string name() const override { return "GeluAct8Backward"; }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return none(1);
-    return {gelu_grad_op().call(grads[0], get(0), get(1))};
+    return {gelu_grad_op().call(grads[0], get(0), get(1), get(2))};
   }
 };
 
-struct LinearNode : public TokenNode {          // w, q, e
+struct LinearNode : public TokenNode {          // w, q, e, tie
   int64_t groups = 0;
   std::string name() const override { return "LinearAct8Backward"; }
   variable_list apply(variable_list&& grads) override {
@@ -813,7 +823,7 @@ struct LinearNode : public TokenNode {          // w, q, e
                           task_should_compute_output(1),
                           task_should_compute_output(2)};
     auto [dx, dw, db] =
-        linear_grad_op().call(grads[0], get(0), get(1), get(2), groups,
+        linear_grad_op().call(grads[0], get(0), get(1), get(2), get(3), groups,
                               want[0], want[1], want[2]);
     return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
             want[2] ? db : Tensor()};
@@ -866,6 +876,16 @@ std::shared_ptr<N> make_node(torch::autograd::edge_list&& edges) {
   return n;
 }
 
+// The gradients are not differentiable again: asking for it raises.
+template <typename... T>
+std::shared_ptr<Node> refuse_second(const char* op, const T&... inputs) {
+  if (!torch::autograd::compute_requires_grad(inputs...)) return nullptr;
+  std::shared_ptr<Node> n(new torch::autograd::NotImplemented(op),
+                          torch::autograd::deleteNode);
+  n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return n;
+}
+
 Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
                    const OptTensor& b, double eps, int64_t groups) {
   std::shared_ptr<NormNode> node;
@@ -889,25 +909,27 @@ Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
 
 // `keep` is set by the first level that needs the 8-bit input; a level below
 // it (the call on a vmap's whole population) must not drop it.
-Int3 gelu_autograd(c10::DispatchKeySet ks, const Tensor& x, bool keep) {
+Int4 gelu_autograd(c10::DispatchKeySet ks, const Tensor& x, bool keep) {
   std::shared_ptr<GeluNode> node;
   refuse_forward_mode("gelu_act8", x);
   if (torch::autograd::compute_requires_grad(x))
     node = make_node<GeluNode>(torch::autograd::collect_next_edges(x));
-  Int3 out;
+  Int4 out;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     out = gelu_op().redispatch(ks & c10::after_autograd_keyset, x,
                                keep || node != nullptr);
   }
   if (node) {
-    node->keep({std::get<1>(out), std::get<2>(out)});
+    torch::autograd::set_history(
+        std::get<3>(out), refuse_second("gelu_act8's gradient", x));
+    node->keep({std::get<1>(out), std::get<2>(out), std::get<3>(out)});
     torch::autograd::set_history(std::get<0>(out), node);
   }
   return out;
 }
 
-Int3 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
+Int4 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
                      const OptTensor& b, bool keep, int64_t groups) {
   std::shared_ptr<LinearNode> node;
   const Tensor bt = or_undefined(b);
@@ -915,7 +937,7 @@ Int3 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
   if (torch::autograd::compute_requires_grad(x, w, bt))
     node =
         make_node<LinearNode>(torch::autograd::collect_next_edges(x, w, bt));
-  Int3 out;
+  Int4 out;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     out = linear_op().redispatch(
@@ -924,7 +946,9 @@ Int3 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
   }
   if (node) {
     node->groups = groups;
-    node->keep({w, std::get<1>(out), std::get<2>(out)});
+    if (auto n = refuse_second("linear_act8's gradient", x))
+      torch::autograd::set_history(std::get<3>(out), n);
+    node->keep({w, std::get<1>(out), std::get<2>(out), std::get<3>(out)});
     torch::autograd::set_history(std::get<0>(out), node);
   }
   return out;
@@ -954,16 +978,6 @@ Int3 loss_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
   return out;
 }
 
-// The gradients are not differentiable again: asking for it raises.
-template <typename... T>
-std::shared_ptr<Node> refuse_second(const char* op, const T&... inputs) {
-  if (!torch::autograd::compute_requires_grad(inputs...)) return nullptr;
-  std::shared_ptr<Node> n(new torch::autograd::NotImplemented(op),
-                          torch::autograd::deleteNode);
-  n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
-  return n;
-}
-
 Int3 with_history(Int3 out, const std::shared_ptr<Node>& n) {
   if (n) {
     torch::autograd::set_history(std::get<0>(out), n);
@@ -985,23 +999,27 @@ Int3 norm_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
 }
 
 Tensor gelu_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
-                          const Tensor& q, const Tensor& e) {
-  auto n = refuse_second("gelu_act8's gradient", dy);
+                          const Tensor& q, const Tensor& e,
+                          const Tensor& tie) {
+  auto n = refuse_second("gelu_act8's gradient", dy, tie);
   at::AutoDispatchBelowADInplaceOrView guard;
-  Tensor out =
-      gelu_grad_op().redispatch(ks & c10::after_autograd_keyset, dy, q, e);
+  Tensor out = gelu_grad_op().redispatch(ks & c10::after_autograd_keyset, dy,
+                                         q, e, tie);
   if (n) torch::autograd::set_history(out, n);
   return out;
 }
 
 Int3 linear_grad_autograd(c10::DispatchKeySet ks, const Tensor& dy,
                           const Tensor& w, const Tensor& q, const Tensor& e,
-                          int64_t groups, bool wx, bool ww, bool wb) {
-  auto n = refuse_second("linear_act8's gradient", dy, w);
+                          const Tensor& tie, int64_t groups, bool wx, bool ww,
+                          bool wb) {
+  // only the weight's gradient depends on the layer's input
+  auto n = refuse_second("linear_act8's gradient", dy, w,
+                         ww ? tie : Tensor());
   at::AutoDispatchBelowADInplaceOrView guard;
   return with_history(
       linear_grad_op().redispatch(ks & c10::after_autograd_keyset, dy, w, q, e,
-                                  groups, wx, ww, wb), n);
+                                  tie, groups, wx, ww, wb), n);
 }
 
 Int3 loss_grad_autograd(c10::DispatchKeySet ks, const Tensor& grad,
@@ -1069,6 +1087,15 @@ struct Level {
   Tensor close(const Tensor& t, bool batched = true) const {
     return batched ? fn::makeBatched(t, 0, level) : t;
   }
+  // a tie has no client axis
+  Tensor strip(const Tensor& t) const {
+    Dim d;
+    return open(t, d);
+  }
+  Int4 close_tied(const Int4& t, bool kept) const {
+    return {close(std::get<0>(t)), close(std::get<1>(t), kept),
+            close(std::get<2>(t), kept), std::get<3>(t)};
+  }
   Int3 close(const Int3& t, bool a, bool b, bool c) const {
     return {close(std::get<0>(t), a), close(std::get<1>(t), b),
             close(std::get<2>(t), c)};
@@ -1105,22 +1132,24 @@ Int3 norm_grad_vmap(const Tensor& dy, const Tensor& x, const OptTensor& w,
                           v.all(rstd), v.size, params), true, params, params);
 }
 
-Int3 gelu_vmap(const Tensor& x, bool keep) {
+Int4 gelu_vmap(const Tensor& x, bool keep) {
   Level v;
   if (!v.has(x)) return gelu_op().call(x, keep);
-  Int3 out = gelu_op().call(v.all(x), keep);
+  Int4 out = gelu_op().call(v.all(x), keep);
   const bool kept = std::get<1>(out).numel() == std::get<0>(out).numel();
-  return v.close(out, true, kept, kept);
+  return v.close_tied(out, kept);
 }
 
-Tensor gelu_grad_vmap(const Tensor& dy, const Tensor& q, const Tensor& e) {
+Tensor gelu_grad_vmap(const Tensor& dy, const Tensor& q, const Tensor& e,
+                      const Tensor& tie) {
   Level v;
   if (!v.has(dy) && !v.has(q) && !v.has(e))
-    return gelu_grad_op().call(dy, q, e);
-  return v.close(gelu_grad_op().call(v.all(dy), v.all(q), v.all(e)));
+    return gelu_grad_op().call(dy, q, e, tie);
+  return v.close(gelu_grad_op().call(v.all(dy), v.all(q), v.all(e),
+                                     v.strip(tie)));
 }
 
-Int3 linear_vmap(const Tensor& x, const Tensor& w, const OptTensor& b,
+Int4 linear_vmap(const Tensor& x, const Tensor& w, const OptTensor& b,
                  bool keep, int64_t groups) {
   Level v;
   if (!v.has(x) && !v.has(w) && !v.has(b))
@@ -1128,23 +1157,24 @@ Int3 linear_vmap(const Tensor& x, const Tensor& w, const OptTensor& b,
   refuse_nested(groups, "linear_act8");
   const bool own = v.has(w) || v.has(b);
   const Tensor xa = v.all(x);
-  Int3 out = linear_op().call(xa, own ? v.all(w) : w, own ? v.all(b) : b, keep,
+  Int4 out = linear_op().call(xa, own ? v.all(w) : w, own ? v.all(b) : b, keep,
                               own ? v.size : 0);
   const bool kept = std::get<1>(out).dim() == xa.dim();
-  return v.close(out, true, kept, kept);
+  return v.close_tied(out, kept);
 }
 
 Int3 linear_grad_vmap(const Tensor& dy, const Tensor& w, const Tensor& q,
-                      const Tensor& e, int64_t groups, bool wx, bool ww,
-                      bool wb) {
+                      const Tensor& e, const Tensor& tie, int64_t groups,
+                      bool wx, bool ww, bool wb) {
   Level v;
   if (!v.has(dy) && !v.has(w) && !v.has(q) && !v.has(e))
-    return linear_grad_op().call(dy, w, q, e, groups, wx, ww, wb);
+    return linear_grad_op().call(dy, w, q, e, tie, groups, wx, ww, wb);
   refuse_nested(groups, "linear_act8");
   return v.close(
       linear_grad_op().call(v.all(dy), v.param(w),
                             ww ? v.all(q) : v.param(q),
-                            ww ? v.all(e) : v.param(e), v.size, wx, ww, wb),
+                            ww ? v.all(e) : v.param(e), v.strip(tie), v.size,
+                            wx, ww, wb),
       wx, ww, wb);
 }
 
@@ -1204,12 +1234,13 @@ TORCH_LIBRARY(blades_amd, m) {
         "-> (Tensor, Tensor, Tensor)");
   m.def("layer_norm_grad(Tensor dy, Tensor x, Tensor? w, Tensor mean, "
         "Tensor rstd, int groups, bool params) -> (Tensor, Tensor, Tensor)");
-  m.def("gelu_act8(Tensor x, bool keep) -> (Tensor, Tensor, Tensor)");
-  m.def("gelu_act8_grad(Tensor dy, Tensor q, Tensor e) -> Tensor");
+  m.def("gelu_act8(Tensor x, bool keep) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("gelu_act8_grad(Tensor dy, Tensor q, Tensor e, Tensor tie) -> Tensor");
   m.def("linear_act8(Tensor x, Tensor w, Tensor? b, bool keep, int groups) "
-        "-> (Tensor, Tensor, Tensor)");
+        "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_act8_grad(Tensor dy, Tensor w, Tensor q, Tensor e, "
-        "int groups, bool want_x, bool want_w, bool want_b) "
+        "Tensor tie, int groups, bool want_x, bool want_w, bool want_b) "
         "-> (Tensor, Tensor, Tensor)");
   m.def("linear_cross_entropy(Tensor x, Tensor w, Tensor target, Tensor? b, "
         "int ignore, int reduction, int groups) -> (Tensor, Tensor, Tensor)");

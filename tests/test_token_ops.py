@@ -976,3 +976,75 @@ def test_captured_population_step(fn, rows):
         torch.cuda.synchronize()
         for a, r in zip(outs[i % 2], want):
             assert torch.equal(a, r)
+
+
+# ------------------------------------------- what is refused at every level
+
+def _calls(device):
+    """name -> (scalar function of (x, w), x, w); the upstream gradient of
+    each operator is a constant."""
+    x, w, y, b = loss_inputs(5, 16, 16, torch.float32, device)
+    return {"norm": lambda x, w: ops.layer_norm(x, w[0]).sum(),
+            "loss": lambda x, w: ops.linear_cross_entropy(x, w, y, b),
+            "gelu": lambda x, w: ops.gelu_act8(x).sum(),
+            "linear": lambda x, w: ops.linear_act8(x, w, b).sum()}, x, w
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", ["norm", "loss", "gelu", "linear"])
+def test_second_gradient_refused_with_constant_upstream(device, fn):
+    """A gradient penalty: the first gradients come, their own raise."""
+    calls, x, w = _calls(device)
+    x.requires_grad_(), w.requires_grad_()
+    leaves = (x,) if fn == "gelu" else (x, w)
+    want = torch.autograd.grad(calls[fn](x, w), leaves)
+    out = calls[fn](x, w)
+    first = torch.autograd.grad(out, leaves, create_graph=True)
+    for a, r in zip(first, want):
+        assert torch.equal(a, r)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.autograd.grad(out + sum(g.square().sum() for g in first), x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", ["norm", "loss", "gelu"])
+@pytest.mark.parametrize("clients", [0, 3])
+def test_nested_func_grad_refused(device, fn, clients):
+    calls, x, w = _calls(device)
+
+    def penalty(x):
+        return torch.func.grad(lambda z: calls[fn](z, w))(x).square().sum()
+    outer = torch.func.grad(penalty)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        if clients:
+            torch.func.vmap(outer)(x.expand(clients, *x.shape))
+        else:
+            outer(x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", ["norm", "loss", "linear"])
+@pytest.mark.parametrize("clients", [0, 3])
+def test_mixed_second_gradient_refused(device, fn, clients):
+    """The weight's gradient, differentiated by the input."""
+    calls, x, w = _calls(device)
+
+    def penalty(x, w):
+        return torch.func.grad(lambda u: calls[fn](x, u))(w).square().sum()
+    outer = torch.func.grad(penalty)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        if clients:
+            torch.func.vmap(outer, in_dims=(0, None))(
+                x.expand(clients, *x.shape), w)
+        else:
+            outer(x, w)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_input_gradient_of_linear_is_constant_in_the_input(device):
+    """dx = dy w does not depend on x: nothing is missing from its second
+    gradient, and it is not refused."""
+    x, w, _, b = loss_inputs(5, 16, 16, torch.float32, device)
+    g = torch.func.grad(lambda x: torch.func.grad(
+        lambda z: ops.linear_act8(z, w, b).sum())(x).square().sum())(x)
+    assert torch.equal(g, torch.zeros_like(g))
