@@ -76,6 +76,9 @@ class EncoderLayer(nn.Module):
     x = x + drop_path(mlp(x)).
     """
 
+    # layers pickled before the choice existed have none of their own
+    gelu = staticmethod(F.gelu)
+
     def __init__(self, dim: int, heads: int, mlp_ratio: float,
                  dropout: float, attn_dropout: float, drop_path: float,
                  fused_norm: bool = False, act_bits: int = 32):

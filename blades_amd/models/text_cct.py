@@ -80,6 +80,9 @@ class MaskedEncoderLayer(nn.Module):
     """Pre-norm encoder layer (cct.EncoderLayer topology) with a
     key-padding mask applied inside SDPA."""
 
+    # layers pickled before the choice existed have none of their own
+    gelu = staticmethod(F.gelu)
+
     def __init__(self, dim: int, heads: int, mlp_ratio: float,
                  dropout: float, attn_dropout: float, drop_path: float,
                  fused_norm: bool = False, act_bits: int = 32):

@@ -1,5 +1,7 @@
 """The token operators where the framework uses them: the transformers'
 layers, the simulator's logit-free loss, and a whole step of them together."""
+import pickle
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -87,6 +89,19 @@ def test_registry_takes_the_options():
     m = get_model("vit_lite", fused_norm=True, act_bits=8)
     assert any(isinstance(s, Act8Linear) for s in m.modules())
     assert m(torch.randn(1, 3, 32, 32)).shape == (1, 10)
+
+
+@pytest.mark.parametrize("make", [text_model, image_model])
+def test_layers_pickled_without_the_choice_of_gelu(make):
+    """Models saved whole before layers had a GELU of their own still run."""
+    torch.manual_seed(0)
+    model = make().eval()
+    x, _ = batch(model, "cpu")
+    want = model(x)
+    for m in model.modules():
+        m.__dict__.pop("gelu", None)
+    old = pickle.loads(pickle.dumps(model))
+    assert torch.equal(old(x), want)
 
 
 class TokenDataset:
