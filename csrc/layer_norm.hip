@@ -404,7 +404,8 @@ void norm_params_wide_kernel(NormArgs a) {
 }
 
 // Sums `blocks` partial rows of `width` floats per group.  A block takes 32
-// columns; its 8 row lanes walk the partials and meet in shared memory.
+// columns at a time; its 8 row lanes walk the partials and meet in shared
+// memory.
 // Columns below `split` go to out0, the rest to out1 (either may be null).
 template <typename T>
 __global__ __launch_bounds__(kThreads)
@@ -413,33 +414,37 @@ void join_rows_kernel(const float* __restrict__ partial, long long blocks,
                       long long out0_group, T* out1, Scale scale) {
   __shared__ float part[8][33];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const long long c = (long long)blockIdx.x * 32 + cl;
   const long long g = blockIdx.y;
   const float* p = partial + g * blocks * width;
-  float s = 0.f;
-  if (c < width) {
-    float s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    long long r = rl;
-    for (; r + 24 < blocks; r += 32) {
-      s += p[r * width + c];
-      s1 += p[(r + 8) * width + c];
-      s2 += p[(r + 16) * width + c];
-      s3 += p[(r + 24) * width + c];
+  for (long long c0 = (long long)blockIdx.x * 32; c0 < width;
+       c0 += (long long)gridDim.x * 32) {
+    const long long c = c0 + cl;
+    float s = 0.f;
+    if (c < width) {
+      float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      long long r = rl;
+      for (; r + 24 < blocks; r += 32) {
+        s += p[r * width + c];
+        s1 += p[(r + 8) * width + c];
+        s2 += p[(r + 16) * width + c];
+        s3 += p[(r + 24) * width + c];
+      }
+      for (; r < blocks; r += 8) s += p[r * width + c];
+      s = (s + s1) + (s2 + s3);
     }
-    for (; r < blocks; r += 8) s += p[r * width + c];
-    s = (s + s1) + (s2 + s3);
-  }
-  part[rl][cl] = s;
-  __syncthreads();
-  if (rl == 0 && c < width) {
+    part[rl][cl] = s;
+    __syncthreads();
+    if (rl == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][cl];
-    s *= scale_of(scale, g);
-    if (c < split) {
-      if (out0) out0[g * out0_group + c] = from_f<T>(s);
-    } else if (out1) {
-      out1[g * (width - split) + (c - split)] = from_f<T>(s);
+      for (int i = 1; i < 8; ++i) s += part[i][cl];
+      s *= scale_of(scale, g);
+      if (c < split) {
+        if (out0) out0[g * out0_group + c] = from_f<T>(s);
+      } else if (out1) {
+        out1[g * (width - split) + (c - split)] = from_f<T>(s);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -579,7 +584,7 @@ void backward_t(const NormArgs& a, hipStream_t s) {
   }
   if (a.partial)
     join_rows_kernel<T>
-        <<<dim3((unsigned)ceil_div(2 * a.dim, 32), (unsigned)a.groups),
+        <<<dim3(row_grid(ceil_div(2 * a.dim, 32)), (unsigned)a.groups),
            kThreads, 0, s>>>(a.partial, blocks, 2 * a.dim, a.dim,
                              static_cast<T*>(a.dw), a.dim,
                              static_cast<T*>(a.db), Scale{});
@@ -642,7 +647,7 @@ void colsum(const void* x, void* out, float* partial, long long groups,
 void join_rows(const float* partial, long long groups, long long blocks,
                long long cols, void* out, long long out_group,
                const Scale& scale, DType t, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)groups);
+  const dim3 grid(row_grid(ceil_div(cols, 32)), (unsigned)groups);
   if (t == kF32)
     join_rows_kernel<float><<<grid, kThreads, 0, s>>>(
         partial, blocks, cols, cols, static_cast<float*>(out), out_group,

@@ -10,6 +10,7 @@
 #include <ATen/functorch/PlumbingHelper.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -67,9 +68,8 @@ hipStream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.get_device()).stream();
 }
 
-const void* data(const OptTensor& t) {
-  return t.has_value() ? t->data_ptr() : nullptr;
-}
+// After launches: one that the runtime refused leaves its output unwritten.
+void check_launched() { C10_HIP_CHECK(hipGetLastError()); }
 
 Tensor floats(const Tensor& like, at::IntArrayRef sizes) {
   return at::empty(sizes, like.options().dtype(at::kFloat));
@@ -113,7 +113,10 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward_t(
   a.mean = mean.data_ptr<float>();
   a.rstd = rstd.data_ptr<float>();
   a.eps = (float)eps;
-  if (a.rows > 0) norm_forward(a, t, stream_of(x));
+  if (a.rows > 0) {
+    norm_forward(a, t, stream_of(x));
+    check_launched();
+  }
   return {y, mean, rstd};
 }
 
@@ -151,6 +154,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_t(
     a.db = db.data_ptr();
   }
   norm_backward(a, t, stream_of(x));
+  check_launched();
   return {dx, dw, db};
 }
 
@@ -168,6 +172,7 @@ Tensor colsum_t(const Tensor& x) {
       floats(x, {groups * colsum_blocks(groups, rows, cols), cols});
   colsum(x.data_ptr(), out.data_ptr(), partial.data_ptr<float>(), groups, rows,
          cols, t, stream_of(x));
+  check_launched();
   return out;
 }
 
@@ -207,9 +212,11 @@ std::tuple<Tensor, Tensor> act8_pack_t(const Tensor& x) {
   check_act(x);
   c10::DeviceGuard guard(x.device());
   Packed p = packed_like(x);
-  if (x.numel() > 0)
+  if (x.numel() > 0) {
     act8_pack(x.data_ptr(), p.q.data_ptr<int8_t>(), p.e.data_ptr<uint8_t>(),
               x.numel() / x.size(-1), x.size(-1), dtype_of(x), stream_of(x));
+    check_launched();
+  }
   return {p.q, p.e};
 }
 
@@ -224,12 +231,14 @@ std::tuple<Tensor, Tensor, Tensor> gelu_forward_t(const Tensor& x, bool keep) {
     p.q = at::empty({0}, x.options().dtype(at::kChar));
     p.e = at::empty({0}, x.options().dtype(at::kByte));
   }
-  if (x.numel() > 0)
+  if (x.numel() > 0) {
     gelu_forward(x.data_ptr(), y.data_ptr(),
                  keep ? p.q.data_ptr<int8_t>() : nullptr,
                  keep ? p.e.data_ptr<uint8_t>() : nullptr,
                  x.numel() / x.size(-1), x.size(-1), dtype_of(x),
                  stream_of(x));
+    check_launched();
+  }
   return {y, p.q, p.e};
 }
 
@@ -239,10 +248,12 @@ Tensor gelu_backward_t(const Tensor& dy, const Tensor& q, const Tensor& e) {
   TORCH_CHECK(q.sizes() == dy.sizes(), "q must have dy's shape");
   c10::DeviceGuard guard(dy.device());
   Tensor dx = at::empty_like(dy);
-  if (dy.numel() > 0)
+  if (dy.numel() > 0) {
     gelu_backward(dy.data_ptr(), q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(),
                   dx.data_ptr(), dy.numel() / dy.size(-1), dy.size(-1),
                   dtype_of(dy), stream_of(dy));
+    check_launched();
+  }
   return dx;
 }
 
@@ -272,6 +283,7 @@ void run_gemm(Gemm& g, const Tensor& like) {
   const hipStream_t s = stream_of(like);
   if (splits == 1) {
     gemm(g, s);
+    check_launched();
     return;
   }
   Tensor partial = floats(like, {splits, g.groups, g.m, g.n});
@@ -281,6 +293,7 @@ void run_gemm(Gemm& g, const Tensor& like) {
   TORCH_CHECK(g.out_ld == g.n, "a joined output's rows have no gaps");
   join_partials(g.partial, splits, g.groups, g.m, g.n, g.out, g.out_group,
                 g.bias, g.bias_group, g.tout, s);
+  check_launched();
 }
 
 // y[g] = x[g] w' + b
@@ -449,6 +462,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_forward_t(
                reduction ? sums.data_ptr() : nullptr,
                reduction ? loss.data_ptr<float>() : nullptr,
                count.data_ptr<float>(), reduction == 2, stream_of(x));
+  check_launched();
   return {reduction ? loss : rows, lse, count};
 }
 
@@ -573,6 +587,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
   if (want_x && parts)
     join_partials(xsum.data_ptr<float>(), splits, l.groups, l.rows, l.dim,
                   dx.data_ptr(), l.rows * l.dim, nullptr, 0, l.t, s);
+  check_launched();
   return {dx, dw, db};
 }
 

@@ -1048,3 +1048,26 @@ def test_input_gradient_of_linear_is_constant_in_the_input(device):
     g = torch.func.grad(lambda x: torch.func.grad(
         lambda z: ops.linear_act8(z, w, b).sum())(x).square().sum())(x)
     assert torch.equal(g, torch.zeros_like(g))
+
+
+@gpu
+def test_norm_widest_rows_parameter_gradients():
+    """One row of 2**28 values: the kernel that joins the parameters'
+    gradients covers them all.  With one row db is dy, bit for bit, and dw is
+    dy * h: a rounding of each factor and of the product, and h's own error,
+    (n + 8) U of it in the worst order of its sums."""
+    n = 1 << 28
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(1, n, generator=g, device="cuda")
+    dy = torch.randn(1, n, generator=g, device="cuda")
+    w = torch.ones(n, device="cuda", requires_grad=True)
+    b = torch.zeros(n, device="cuda", requires_grad=True)
+    y = ops.layer_norm(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    assert torch.equal(db, dy[0])
+    # y is h here: dw differs from dy * y by the product's rounding alone
+    y = y.detach()
+    assert bool(((dw - dy[0] * y[0]).abs()
+                 <= 4 * U * (dy[0] * y[0]).abs()).all())
+    assert abs(float(y.double().mean())) < 1e-3
+    assert abs(float(y.double().square().mean()) - 1) < 1e-3
