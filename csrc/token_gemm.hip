@@ -6,10 +6,14 @@
 //     (act8.hip), whose stored values are exact in bf16;
 //   * order: contraction along the rows ([m][k]) or across them ([k][m]).
 //
-// fp32: x = hi + mid + lo by truncation is exact (8 + 8 + 8 bits), and the
-// six products hi*hi, hi*mid, mid*hi, hi*lo, mid*mid, lo*hi leave out only
-// terms below 2^-23 of |a||b|, so results are fp32's; six bf16 products per
-// multiplication have 2.6 times the rate of the fp32 matrix instruction.
+// fp32: x = hi + mid + lo, each the nearest bf16 to what is left, is exact:
+// |mid| <= 2^-8 and |lo| <= 2^-17 of a power of two not above |x|.  The six
+// products hi*hi, hi*mid, mid*hi, hi*lo, mid*mid, lo*hi leave out mid*lo,
+// lo*mid and lo*lo, at most 2^-24 of |a||b| (half a step of fp32) and of
+// either sign.  (Parts cut off instead of rounded are twice and four times as
+// large and have the operand's sign: up to 2^-21 left out, always towards
+// zero.)  Six bf16 products per multiplication have 2.6 times the rate of the
+// fp32 matrix instruction.
 // A value that is not finite makes its results NaN (inf - inf in the parts).
 //
 // A block owns 256 x 256, 128 x 128 or 64 x 64 of the output (tiling() below
@@ -96,22 +100,27 @@ struct Params {
   Scale scale;            // of what STORE writes
 };
 
+// The nearest bf16 to two floats, packed; a and b keep what is left.
+__device__ __forceinline__ uint32_t take_bf16(float na, float nb, float& a,
+                                              float& b) {
+  const bf16x2 t = {(bf16)na, (bf16)nb};
+  const uint32_t u = __builtin_bit_cast(uint32_t, t);
+  a -= __uint_as_float(u << 16);
+  b -= __uint_as_float(u & 0xffff0000u);
+  return u;
+}
+
 // Three bf16 parts of 8 floats, packed in pairs.
 __device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&o)[3]) {
+  // bf16's largest value: what would round beyond it leaves more to mid
+  constexpr float kMost = 0x1.fep127f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t h[2], m[2], l[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float v = x[2 * j + i];
-      h[i] = __float_as_uint(v);
-      const float r = v - __uint_as_float(h[i] & 0xffff0000u);
-      m[i] = __float_as_uint(r);
-      l[i] = __float_as_uint(r - __uint_as_float(m[i] & 0xffff0000u));
-    }
-    o[0][j] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302u);
-    o[1][j] = __builtin_amdgcn_perm(m[1], m[0], 0x07060302u);
-    o[2][j] = __builtin_amdgcn_perm(l[1], l[0], 0x07060302u);
+    float a = x[2 * j], b = x[2 * j + 1];
+    o[0][j] = take_bf16(__builtin_amdgcn_fmed3f(a, -kMost, kMost),
+                        __builtin_amdgcn_fmed3f(b, -kMost, kMost), a, b);
+    o[1][j] = take_bf16(a, b, a, b);
+    o[2][j] = take_bf16(a, b, a, b);
   }
 }
 

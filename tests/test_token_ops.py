@@ -1071,3 +1071,33 @@ def test_norm_widest_rows_parameter_gradients():
                  <= 4 * U * (dy[0] * y[0]).abs()).all())
     assert abs(float(y.double().mean())) < 1e-3
     assert abs(float(y.double().square().mean()) - 1) < 1e-3
+
+
+# ------------------------------------------------------ fp32 products' bits
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_single_products_keep_fp32(device):
+    """Products of two values whose bits are all set: a product's rounding is
+    U, and a kernel that multiplies in parts adds at most five more roundings
+    of partial sums and U of products left out: 7 U in all, less where sums of
+    parts are exact."""
+    k = torch.arange(1, 2049, dtype=torch.int32)
+    a = (0x3F810000 - k).view(torch.float32)[:, None].to(device)
+    got = ops.linear_act8(a, a).double()
+    want = a.double() @ a.double().t()
+    assert ((got - want) / want).abs().max() <= 7 * U
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_single_products_have_no_bias(device):
+    """Errors of independent products, each at most 7 U, average out: over
+    n of them beyond 7 U sqrt(2 ln(2e9) / n) = 0.18 U once in 1e9 (a mean of
+    bounded variables, Hoeffding)."""
+    n = 65535
+    g = torch.Generator().manual_seed(0)
+    a, b = (torch.randint(0x3F800000, 0x40000000, (n, 1, 1), generator=g,
+                          dtype=torch.int32).view(torch.float32).to(device)
+            for _ in range(2))
+    got = torch.func.vmap(ops.linear_act8)(a, b).double()
+    want = a.double() * b.double()
+    assert abs(((got - want) / want).mean()) <= 0.18 * U
