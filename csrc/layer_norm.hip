@@ -437,7 +437,7 @@ void join_rows_kernel(const float* __restrict__ partial, long long blocks,
     if (rl == 0 && c < width) {
 #pragma unroll
       for (int i = 1; i < 8; ++i) s += part[i][cl];
-      s *= scale_of(scale, g);
+      s = scaled(s, scale_of(scale, g));
       if (c < split) {
         if (out0) out0[g * out0_group + c] = from_f<T>(s);
       } else if (out1) {

@@ -94,6 +94,12 @@ __device__ __forceinline__ float scale_of(const Scale& s, long long g) {
   return s.den[g] == 0.f ? 0.f : s.num[g] / s.den[g];
 }
 
+// v * s, and 0 where v is 0: what nothing counted towards stays without a
+// gradient under a factor that is not finite.
+__device__ __forceinline__ float scaled(float v, float s) {
+  return v == 0.f ? 0.f : v * s;
+}
+
 // Sum over groups of W neighbouring lanes (W a power of two up to 64); every
 // lane gets it, in an order that does not depend on timing.
 template <int W> __device__ __forceinline__ float lanes_sum(float v) {

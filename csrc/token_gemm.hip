@@ -607,6 +607,7 @@ void gemm_kernel(Params p) {
 
   if constexpr (E == STORE) {
     const float scale = scale_of(p.scale, g);
+    const bool finite = fabsf(scale) < INFINITY;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const int n = n0 + j * 32 + (lane & 31);
@@ -621,7 +622,8 @@ void gemm_kernel(Params p) {
         for (int r = 0; r < 16; ++r) {
           const int m = m0 + i * 32 + acc_row(r, lane);
           if (m >= M) continue;
-          const float v = fmaf(acc[i][j][r], scale, bias);
+          const float v = finite ? fmaf(acc[i][j][r], scale, bias)
+                                 : scaled(acc[i][j][r], scale) + bias;
           if (p.partial) {
             float* o = p.partial
                 + (((long long)split * gridDim.z + g) * M + m) * N + n;

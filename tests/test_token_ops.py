@@ -1101,3 +1101,26 @@ def test_linear_single_products_have_no_bias(device):
     got = torch.func.vmap(ops.linear_act8)(a, b).double()
     want = a.double() * b.double()
     assert abs(((got - want) / want).mean()) <= 0.18 * U
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_loss_non_finite_upstream_leaves_ignored_rows(device, dtype, reduction,
+                                                      bad):
+    """Rows that do not count have no gradient whatever comes from above."""
+    x, w, y, b = loss_inputs(6, 16, 50, dtype, device)       # y[2] is ignored
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    out = ops.linear_cross_entropy(x, w, y, b, reduction=reduction)
+    up = torch.tensor(bad, device=device)
+    dx, dw, db = torch.autograd.grad(out, (x, w, b), up)
+    assert torch.equal(dx[2], torch.zeros_like(dx[2]))
+    assert not dx[[0, 1, 3, 4, 5]].isfinite().any()
+    assert not dw.isfinite().any() and not db.isfinite().any()
+    # nothing counts: a sum has no gradient at all
+    if reduction == "sum":
+        out = ops.linear_cross_entropy(x, w, torch.full_like(y, -100), b,
+                                       reduction="sum")
+        for g in torch.autograd.grad(out, (x, w, b), up):
+            assert torch.equal(g, torch.zeros_like(g))
