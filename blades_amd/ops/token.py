@@ -14,8 +14,10 @@ below, which have the same rules.  Every operator runs under
 ``torch.func.grad`` and ``torch.func.vmap`` in either nesting: a vmapped call is ONE launch over all
 clients ("groups" below), with shared or per-client parameters, and
 ``vmap(grad(...))`` gets the parameters' gradients per client from the
-kernels.  A vmap inside a vmap whose parameters or gradients are per client at
-both levels is refused.  The operators' gradients are not differentiable
+kernels.  Vmaps nest as long as the inner one's clients share their parameters
+and no gradient is taken per client at both levels; a loss that is summed or
+averaged per client needs the parameters shared at both.  Other nestings are
+refused.  The operators' gradients are not differentiable
 again.
 """
 from __future__ import annotations
@@ -287,11 +289,22 @@ class _HeadLoss(Function):
 
     @staticmethod
     def vmap(info, in_dims, x, w, b, target, ignore, reduction, groups):
-        _refuse_nested(groups, "linear_cross_entropy")
         n = info.batch_size
         x = _batched(x, in_dims[0], n)
         target = _batched(target, in_dims[3], n)
-        if in_dims[1] is not None or in_dims[2] is not None:
+        own = in_dims[1] is not None or in_dims[2] is not None
+        if not own and not groups and reduction == 0:
+            # rows of shared parameters: no client is told from another
+            return (_HeadLoss.apply(x, w, b, target, ignore, reduction, 0),
+                    (0, 0, None))
+        if not own and groups and w.dim() == 2 and (b is None or b.dim() == 1):
+            # clients of an inner vmap who share the parameters with these:
+            # as many groups as pairs
+            out = _HeadLoss.apply(x.flatten(0, 1), w, b, target.flatten(0, 1),
+                                  ignore, reduction, n * groups)
+            return tuple(t.unflatten(0, (n, groups)) for t in out), (0, 0, 0)
+        _refuse_nested(groups, "linear_cross_entropy")
+        if own:
             w, b = _batched(w, in_dims[1], n), _batched(b, in_dims[2], n)
         return (_HeadLoss.apply(x, w, b, target, ignore, reduction, n),
                 (0, 0, 0))

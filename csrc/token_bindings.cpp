@@ -1199,8 +1199,25 @@ Int3 loss_vmap(const Tensor& x, const Tensor& w, const Tensor& target,
   Level v;
   if (!v.has(x) && !v.has(w) && !v.has(target) && !v.has(b))
     return loss_op().call(x, w, target, b, ignore, reduction, groups);
-  refuse_nested(groups, "linear_cross_entropy");
   const bool own = v.has(w) || v.has(b);
+  if (!own && groups == 0 && reduction == 0) {
+    // rows of shared parameters: no client is told from another
+    const Int3 out =
+        loss_op().call(v.all(x), w, v.all(target), b, ignore, reduction, 0);
+    return v.close(out, true, true, false);
+  }
+  if (!own && groups && w.dim() == 2 && (!b.has_value() || b->dim() == 1)) {
+    // clients of an inner vmap who share the parameters with these: as many
+    // groups as pairs
+    const int64_t n = v.size;
+    const Int3 out =
+        loss_op().call(v.all(x).flatten(0, 1), w, v.all(target).flatten(0, 1),
+                       b, ignore, reduction, n * groups);
+    auto pairs = [&](const Tensor& t) { return t.unflatten(0, {n, groups}); };
+    return v.close({pairs(std::get<0>(out)), pairs(std::get<1>(out)),
+                    pairs(std::get<2>(out))}, true, true, true);
+  }
+  refuse_nested(groups, "linear_cross_entropy");
   return v.close(
       loss_op().call(v.all(x), own ? v.all(w) : w, v.all(target),
                      own ? v.all(b) : b, ignore, reduction, v.size),

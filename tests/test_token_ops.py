@@ -1124,3 +1124,73 @@ def test_loss_non_finite_upstream_leaves_ignored_rows(device, dtype, reduction,
                                        reduction="sum")
         for g in torch.autograd.grad(out, (x, w, b), up):
             assert torch.equal(g, torch.zeros_like(g))
+
+
+# ------------------------------------------------- shared parameters, nested
+
+def loss_sum_fn(w, b, x, y):
+    return ops.linear_cross_entropy(x, w, y, b, reduction="sum")
+
+
+def loss_rows_fn(w, b, x, y):
+    return ops.linear_cross_entropy(x, w, y, b, reduction="none")
+
+
+NESTED = [loss_fn, loss_sum_fn, loss_rows_fn, norm_fn, gelu_linear_fn]
+
+
+def nested_inputs(fn, device):
+    """Shared w, b; x, y with two client axes (2, 3); an upstream gradient."""
+    w, b, x, y, _ = population(
+        fn if fn in (norm_fn, gelu_linear_fn) else loss_fn, 6, device)
+    w, b = w[0].contiguous(), b[0].contiguous()
+    out = torch.stack([fn(w, b, x[i], y[i]) for i in range(6)])
+    up = rand(*out.shape, device=device, seed=11)
+    nest = lambda t: t.unflatten(0, (2, 3))
+    return w, b, x, y, up, nest
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", NESTED)
+def test_nested_vmap_of_shared_parameters(device, fn):
+    w, b, x, y, up, nest = nested_inputs(fn, device)
+    dims = (None, None, 0, 0)
+    twice = torch.func.vmap(torch.func.vmap(fn, in_dims=dims), in_dims=dims)
+    want = torch.stack([fn(w, b, x[i], y[i]) for i in range(6)])
+    close(twice(w, b, nest(x), nest(y)), nest(want))
+    # another axis order, and the inner axis missing from the targets
+    got = torch.func.vmap(torch.func.vmap(fn, in_dims=dims),
+                          in_dims=(None, None, 1, 1))(
+        w, b, nest(x).movedim(0, 1), nest(y).movedim(0, 1))
+    close(got, nest(want))
+    # the gradients of everything, summed over both axes for the parameters
+    def total(w, b, x):
+        return (twice(w, b, nest(x), nest(y)) * nest(up)).sum()
+    got = torch.func.grad(total, argnums=(0, 1, 2))(w, b, x)
+    leaves = [t.clone().requires_grad_() for t in (w, b, x)]
+    out = torch.stack([fn(leaves[0], leaves[1], leaves[2][i], y[i])
+                       for i in range(6)])
+    for g, r in zip(got, torch.autograd.grad((out * up).sum(), leaves)):
+        close(g, r)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", NESTED)
+def test_gradient_between_vmaps_of_shared_parameters(device, fn):
+    """vmap(grad(vmap(...))): the outer clients' gradients of their inner
+    populations."""
+    w, b, x, y, up, nest = nested_inputs(fn, device)
+
+    def inner(w, b, x, y, up):
+        out = torch.func.vmap(fn, in_dims=(None, None, 0, 0))(w, b, x, y)
+        return (out * up).sum()
+    step = torch.func.grad(inner, argnums=(0, 1, 2))
+    got = torch.func.vmap(step, in_dims=(None, None, 0, 0, 0))(
+        w, b, nest(x), nest(y), nest(up))
+    for i in range(2):
+        leaves = [t.clone().requires_grad_() for t in (w, b, nest(x)[i])]
+        out = torch.stack([fn(leaves[0], leaves[1], leaves[2][k],
+                              nest(y)[i][k]) for k in range(3)])
+        want = torch.autograd.grad((out * nest(up)[i]).sum(), leaves)
+        for g, r in zip(got, want):
+            close(g[i], r)
