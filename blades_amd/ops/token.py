@@ -86,6 +86,16 @@ def _param_batched(t, dim):
     return t if t is None or dim is None else t.movedim(dim, 0)
 
 
+def _shared(p: Optional[Tensor], groups: int, dims: int) -> bool:
+    """Of a call with groups: whether a parameter of ``dims`` dimensions is
+    shared, so that its gradients per client have to be summed."""
+    return bool(groups) and p is not None and p.dim() == dims
+
+
+def _summed(grad, shared: bool):
+    return grad.sum(0) if shared else grad
+
+
 def _refuse_nested(groups: int, op: str) -> None:
     if groups:
         raise NotImplementedError(
@@ -147,8 +157,8 @@ class _NormGrad(_NoSecond):
 
 
 class _Norm(Function):
-    # groups: 0, or the number of clients on x's first axis with parameters of
-    # their own in w and b
+    # groups: 0, or the number of clients on x's first axis; each of w and b
+    # is then per client or shared
 
     @staticmethod
     def forward(x, w, b, eps, groups):
@@ -166,6 +176,7 @@ class _Norm(Function):
         ctx.save_for_backward(x, w, mean, rstd)
         ctx.groups = groups
         ctx.has_b = b is not None
+        ctx.shared = _shared(w, groups, 1), _shared(b, groups, 1)
 
     @staticmethod
     def backward(ctx, dy, _mean, _rstd):
@@ -174,8 +185,8 @@ class _Norm(Function):
         need_b = ctx.has_b and ctx.needs_input_grad[2]
         dx, dw, db = _NormGrad.apply(dy, x, w, mean, rstd, ctx.groups,
                                      need_w or need_b)
-        return (dx, dw if need_w else None, db if need_b else None, None,
-                None)
+        return (dx, _summed(dw, ctx.shared[0]) if need_w else None,
+                _summed(db, ctx.shared[1]) if need_b else None, None, None)
 
     @staticmethod
     def vmap(info, in_dims, x, w, b, eps, groups):
@@ -183,8 +194,8 @@ class _Norm(Function):
         n = info.batch_size
         x = _batched(x, in_dims[0], n)
         if in_dims[1] is not None or in_dims[2] is not None:
-            w, b, groups = (_batched(w, in_dims[1], n),
-                            _batched(b, in_dims[2], n), n)
+            w, b, groups = (_param_batched(w, in_dims[1]),
+                            _param_batched(b, in_dims[2]), n)
         return _Norm.apply(x, w, b, eps, groups), (0, 0, 0)
 
 
@@ -273,7 +284,8 @@ class _HeadLoss(Function):
         ignore, reduction, groups = ctx.settings
         wants = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                  b is not None and ctx.needs_input_grad[2])
-        if groups and w.dim() == 2:
+        shared_w, shared_b = _shared(w, groups, 2), _shared(b, groups, 1)
+        if shared_w and (shared_b or b is None):
             # shared parameters: one sum over all clients' rows, each row
             # with its client's share of the upstream gradient
             if reduction == 2:
@@ -282,10 +294,13 @@ class _HeadLoss(Function):
                 ones = (1,) * (target.dim() - 1)
                 grad = grad.view(-1, *ones).expand(target.shape)
             reduction, groups, count = 0, 0, count[:1]
+            shared_w = shared_b = False
         dx, dw, db = _HeadLossGrad.apply(grad, x, w, b, target, lse, count,
                                          ignore, reduction, groups, wants)
-        return (dx if wants[0] else None, dw if wants[1] else None,
-                db if wants[2] else None, None, None, None, None)
+        return (dx if wants[0] else None,
+                _summed(dw, shared_w) if wants[1] else None,
+                _summed(db, shared_b) if wants[2] else None, None, None, None,
+                None)
 
     @staticmethod
     def vmap(info, in_dims, x, w, b, target, ignore, reduction, groups):
@@ -304,8 +319,7 @@ class _HeadLoss(Function):
                                   ignore, reduction, n * groups)
             return tuple(t.unflatten(0, (n, groups)) for t in out), (0, 0, 0)
         _refuse_nested(groups, "linear_cross_entropy")
-        if own:
-            w, b = _batched(w, in_dims[1], n), _batched(b, in_dims[2], n)
+        w, b = _param_batched(w, in_dims[1]), _param_batched(b, in_dims[2])
         return (_HeadLoss.apply(x, w, b, target, ignore, reduction, n),
                 (0, 0, 0))
 
@@ -498,17 +512,27 @@ class _Linear8(Function):
         ctx.save_for_backward(w, q, e, tie)
         ctx.groups = groups
         ctx.has_b = b is not None
+        ctx.shared = _shared(w, groups, 2), _shared(b, groups, 1)
 
     @staticmethod
     def backward(ctx, dy, _q, _e, _tie):
         w, q, e, tie = ctx.saved_tensors
         wants = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                  ctx.has_b and ctx.needs_input_grad[2])
+        shared_w, shared_b = ctx.shared
+        # a shared weight's gradient is one product over all clients' rows
+        apart = shared_w and not shared_b and wants[2]
         # only the weight's gradient depends on the layer's input
-        dx, dw, db = _LinearGrad.apply(dy, w, q, e, tie if wants[1] else None,
-                                       ctx.groups, wants)
+        dx, dw, db = _LinearGrad.apply(
+            dy, w, q, e, tie if wants[1] else None,
+            0 if shared_w else ctx.groups,
+            (wants[0], wants[1], wants[2] and not apart))
+        if apart:
+            db = _LinearGrad.apply(dy, w, q, e, None, ctx.groups,
+                                   (False, False, True))[2]
         return (dx if wants[0] else None, dw if wants[1] else None,
-                db if wants[2] else None, None, None)
+                _summed(db, shared_b and not shared_w) if wants[2] else None,
+                None, None)
 
     @staticmethod
     def vmap(info, in_dims, x, w, b, keep, groups):
@@ -516,8 +540,8 @@ class _Linear8(Function):
         n = info.batch_size
         x = _batched(x, in_dims[0], n)
         if in_dims[1] is not None or in_dims[2] is not None:
-            w, b, groups = (_batched(w, in_dims[1], n),
-                            _batched(b, in_dims[2], n), n)
+            w, b, groups = (_param_batched(w, in_dims[1]),
+                            _param_batched(b, in_dims[2]), n)
         per = 0 if keep else None
         return _Linear8.apply(x, w, b, keep, groups), (0, per, per, None)
 

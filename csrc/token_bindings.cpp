@@ -603,8 +603,8 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
 //                    per-client ones set `groups`
 //
 // `groups`: 0, or the number of clients on the leading axis of the inputs.
-// A gradient op called with groups gives the parameters' gradients per
-// client.
+// With groups each parameter is per client or shared by itself.  A gradient op
+// called with groups gives both parameters' gradients per client.
 //
 // The 8-bit input that GELU and linear layers keep is integers and carries no
 // autograd history.  An empty float tensor, `tie`, goes with it: it has a
@@ -804,8 +804,18 @@ struct TokenNode : public Node {
   variable_list none(size_t n) { return variable_list(n); }
 };
 
+// Of a call with groups: whether a parameter of `dims` dimensions is shared,
+// so that its gradients per client have to be summed.
+bool is_shared(const Tensor& p, int64_t groups, int64_t dims) {
+  return groups && p.defined() && p.dim() == dims;
+}
+Tensor summed(const Tensor& grad, bool shared) {
+  return shared ? grad.sum(0) : grad;
+}
+
 struct NormNode : public TokenNode {            // x, w, mean, rstd
   int64_t groups = 0;
+  bool shared_w = false, shared_b = false;
   std::string name() const override { return "LayerNormBackward"; }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -815,7 +825,8 @@ struct NormNode : public TokenNode {            // x, w, mean, rstd
     auto [dx, dw, db] =
         norm_grad_op().call(grads[0], get(0), or_none(get(1)), get(2), get(3),
                             groups, want_w || want_b);
-    return {dx, want_w ? dw : Tensor(), want_b ? db : Tensor()};
+    return {dx, want_w ? summed(dw, shared_w) : Tensor(),
+            want_b ? summed(db, shared_b) : Tensor()};
   }
 };
 
@@ -830,6 +841,7 @@ struct GeluNode : public TokenNode {            // q, e, tie
 
 struct LinearNode : public TokenNode {          // w, q, e, tie
   int64_t groups = 0;
+  bool shared_w = false, shared_b = false;
   std::string name() const override { return "LinearAct8Backward"; }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -837,16 +849,24 @@ struct LinearNode : public TokenNode {          // w, q, e, tie
     const bool want[3] = {task_should_compute_output(0),
                           task_should_compute_output(1),
                           task_should_compute_output(2)};
+    // a shared weight's gradient is one product over all clients' rows
+    const bool apart = shared_w && !shared_b && want[2];
     auto [dx, dw, db] =
-        linear_grad_op().call(grads[0], get(0), get(1), get(2), get(3), groups,
-                              want[0], want[1], want[2]);
+        linear_grad_op().call(grads[0], get(0), get(1), get(2), get(3),
+                              shared_w ? 0 : groups, want[0], want[1],
+                              want[2] && !apart);
+    if (apart)
+      db = std::get<2>(linear_grad_op().call(grads[0], get(0), get(1), get(2),
+                                             get(3), groups, false, false,
+                                             true));
     return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
-            want[2] ? db : Tensor()};
+            want[2] ? summed(db, shared_b && !shared_w) : Tensor()};
   }
 };
 
 struct LossNode : public TokenNode {            // x, w, target, b, lse, count
   int64_t ignore = 0, reduction = 0, groups = 0;
+  bool shared_w = false, shared_b = false;
   std::string name() const override { return "LinearCrossEntropyBackward"; }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -856,7 +876,8 @@ struct LossNode : public TokenNode {            // x, w, target, b, lse, count
                           task_should_compute_output(2)};
     Tensor grad = grads[0], w = get(1), target = get(2), count = get(5);
     int64_t red = reduction, g = groups;
-    if (g && w.dim() == 2) {
+    const bool own_b = g && !shared_b && get(3).defined();
+    if (shared_w && !own_b) {
       // shared parameters: one sum over all clients' rows, each row with its
       // client's share of the upstream gradient
       if (red == 2) grad = grad / count;
@@ -872,8 +893,9 @@ struct LossNode : public TokenNode {            // x, w, target, b, lse, count
     auto [dx, dw, db] =
         loss_grad_op().call(grad, get(0), w, target, or_none(get(3)), get(4),
                             count, ignore, red, g, want[0], want[1], want[2]);
-    return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
-            want[2] ? db : Tensor()};
+    return {want[0] ? dx : Tensor(),
+            want[1] ? summed(dw, g && shared_w) : Tensor(),
+            want[2] ? summed(db, g && shared_b) : Tensor()};
   }
 };
 
@@ -916,6 +938,8 @@ Int3 norm_autograd(c10::DispatchKeySet ks, const Tensor& x, const OptTensor& w,
   }
   if (node) {
     node->groups = groups;
+    node->shared_w = is_shared(wt, groups, 1);
+    node->shared_b = is_shared(bt, groups, 1);
     node->keep({x, wt, std::get<1>(out), std::get<2>(out)});
     torch::autograd::set_history(std::get<0>(out), node);
   }
@@ -961,6 +985,8 @@ Int4 linear_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
   }
   if (node) {
     node->groups = groups;
+    node->shared_w = is_shared(w, groups, 2);
+    node->shared_b = is_shared(bt, groups, 1);
     if (auto n = refuse_second("linear_act8's gradient", x))
       torch::autograd::set_history(std::get<3>(out), n);
     node->keep({w, std::get<1>(out), std::get<2>(out), std::get<3>(out)});
@@ -987,6 +1013,8 @@ Int3 loss_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w,
     node->ignore = ignore;
     node->reduction = reduction;
     node->groups = groups;
+    node->shared_w = is_shared(w, groups, 2);
+    node->shared_b = is_shared(bt, groups, 1);
     node->keep({x, w, target, bt, std::get<1>(out), std::get<2>(out)});
     torch::autograd::set_history(std::get<0>(out), node);
   }
@@ -1083,9 +1111,6 @@ struct Level {
     shape.insert(shape.begin(), size);
     return v.unsqueeze(0).expand(shape);
   }
-  OptTensor all(const OptTensor& t) const {
-    return t.has_value() ? OptTensor(all(*t)) : t;
-  }
   // client axis first, or left shared
   Tensor param(const Tensor& t) const {
     Dim d;
@@ -1131,8 +1156,8 @@ Int3 norm_vmap(const Tensor& x, const OptTensor& w, const OptTensor& b,
   refuse_nested(groups, "layer_norm");
   const bool own = v.has(w) || v.has(b);
   return v.close(
-      norm_op().call(v.all(x), own ? v.all(w) : w, own ? v.all(b) : b, eps,
-                     own ? v.size : 0), true, true, true);
+      norm_op().call(v.all(x), v.param(w), v.param(b), eps, own ? v.size : 0),
+      true, true, true);
 }
 
 Int3 norm_grad_vmap(const Tensor& dy, const Tensor& x, const OptTensor& w,
@@ -1172,7 +1197,7 @@ Int4 linear_vmap(const Tensor& x, const Tensor& w, const OptTensor& b,
   refuse_nested(groups, "linear_act8");
   const bool own = v.has(w) || v.has(b);
   const Tensor xa = v.all(x);
-  Int4 out = linear_op().call(xa, own ? v.all(w) : w, own ? v.all(b) : b, keep,
+  Int4 out = linear_op().call(xa, v.param(w), v.param(b), keep,
                               own ? v.size : 0);
   const bool kept = std::get<1>(out).dim() == xa.dim();
   return v.close_tied(out, kept);
@@ -1219,8 +1244,8 @@ Int3 loss_vmap(const Tensor& x, const Tensor& w, const Tensor& target,
   }
   refuse_nested(groups, "linear_cross_entropy");
   return v.close(
-      loss_op().call(v.all(x), own ? v.all(w) : w, v.all(target),
-                     own ? v.all(b) : b, ignore, reduction, v.size),
+      loss_op().call(v.all(x), v.param(w), v.all(target), v.param(b), ignore,
+                     reduction, v.size),
       true, true, true);
 }
 

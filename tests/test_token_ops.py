@@ -1194,3 +1194,82 @@ def test_gradient_between_vmaps_of_shared_parameters(device, fn):
         want = torch.autograd.grad((out * nest(up)[i]).sum(), leaves)
         for g, r in zip(got, want):
             close(g[i], r)
+
+
+# ------------------------------- one of weight and bias shared, one per client
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fn", [loss_fn, loss_rows_fn, norm_fn,
+                                gelu_linear_fn])
+@pytest.mark.parametrize("own", ["w", "b"])
+def test_one_parameter_per_client(device, dtype, fn, own):
+    w, b, x, y, up = population(loss_fn if fn is loss_rows_fn else fn, 4,
+                                device, dtype)
+    if fn is loss_rows_fn:
+        up = rand(4, x.shape[1], device=device, seed=3)
+    if own == "w":
+        b = b[:1].expand_as(b)
+    else:
+        w = w[:1].expand_as(w)
+    want = one_by_one(fn, w, b, x, y, up)
+    w_in, b_in = (w, b[0]) if own == "w" else (w[0], b)
+    dims = (0, None, 0) if own == "w" else (None, 0, 0)
+
+    def step(w, b, x, y, up):
+        out, pull = torch.func.vjp(lambda *a: fn(*a, y), w, b, x)
+        return (out, *pull(up))
+    got = torch.func.vmap(step, in_dims=dims + (0, 0))(w_in, b_in, x, y, up)
+    for g, r in zip(got, want):
+        close(g, r, dtype)
+
+    def total(w, b, x):
+        out = torch.func.vmap(fn, in_dims=dims + (0,))(w, b, x, y)
+        return (out * up).sum()
+    leaves = [t.detach().clone().requires_grad_() for t in (w_in, b_in, x)]
+    got = torch.autograd.grad(total(*leaves), leaves)
+    want[1 if own == "b" else 2] = want[1 if own == "b" else 2].float().sum(0)
+    for g, r, t in zip(got, want[1:], leaves):
+        assert g.dtype == dtype
+        close(g.float(), r.float(), dtype)
+
+
+def test_shared_parameters_are_not_repeated(monkeypatch):
+    """A shared parameter reaches the operators' plain forms as it is, also
+    where the other one is per client."""
+    from blades_amd.ops import torch_ref
+    seen = []
+    for name, at in (("norm_forward", (1, 2)), ("loss_forward", (1, 3)),
+                     ("linear_forward", (1, 2))):
+        def spy(*a, _f=getattr(torch_ref, name), _at=at, **kw):
+            seen.append(tuple(a[i].dim() for i in _at))
+            return _f(*a, **kw)
+        monkeypatch.setattr(torch_ref, name, spy)
+    for fn, dims in ((norm_fn, (1, 1)), (loss_fn, (2, 1)),
+                     (gelu_linear_fn, (2, 1))):
+        w, b, x, y, _ = population(fn, 4, "cpu")
+        seen.clear()
+        torch.func.vmap(fn)(w, b, x, y)
+        torch.func.vmap(fn, in_dims=(0, None, 0, 0))(w, b[0], x, y)
+        torch.func.vmap(fn, in_dims=(None, 0, 0, 0))(w[0], b, x, y)
+        torch.func.vmap(fn, in_dims=(None, None, 0, 0))(w[0], b[0], x, y)
+        i, j = dims
+        assert seen == [(i + 1, j + 1), (i + 1, j), (i, j + 1), (i, j)]
+
+
+@gpu
+def test_shared_weight_is_not_copied_per_client():
+    """64 clients' biases on one head of 20 MB: a copy per client would take
+    1.3 GB."""
+    w = rand(20000, 256, device="cuda")
+    b = rand(64, 20000, device="cuda")
+    x = rand(64, 4, 256, device="cuda")
+    y = torch.zeros(64, 4, dtype=torch.int64, device="cuda")
+    for f in (lambda x, b, y: ops.linear_cross_entropy(x, w, y, b),
+              lambda x, b, y: ops.linear_act8(x, w, b)):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        out = torch.func.vmap(f)(x, b, y)
+        assert torch.cuda.max_memory_allocated() - before < 100 << 20
+        del out
