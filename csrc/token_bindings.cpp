@@ -705,24 +705,13 @@ Tensor gelu_grad_cuda(const Tensor& dy, const Tensor& q, const Tensor& e,
   return gelu_backward_t(dy.contiguous(), q.contiguous(), e.contiguous());
 }
 
-// One plain bf16 product is the library's; fp32 and per-client products run
-// the kernels of token_gemm.hip.
-bool plain_product(const Tensor& x, const Tensor& w) {
-  return w.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.numel() > 0;
-}
-
 Int4 linear_cuda(const Tensor& x, const Tensor& w, const OptTensor& b,
                  bool keep, int64_t groups) {
   c10::DeviceGuard guard(x.device());
-  Tensor y;
   auto shape = x.sizes().vec();
   shape.back() = w.size(-2);
-  if (plain_product(x, w) && (!b.has_value() || b->dim() == 1)) {
-    const Tensor x2 = x.reshape({-1, x.size(-1)}), wt = w.t();
-    y = b.has_value() ? at::addmm(*b, x2, wt) : at::mm(x2, wt);
-  } else {
-    y = linear_forward_t(groups3(x, groups), w.contiguous(), contig(b));
-  }
+  const Tensor y =
+      linear_forward_t(groups3(x, groups), w.contiguous(), contig(b));
   Tensor q, e;
   if (keep) {
     std::tie(q, e) = act8_pack_t(x.contiguous());
@@ -743,9 +732,7 @@ Int3 linear_grad_cuda(const Tensor& dy, const Tensor& w, const Tensor& q,
   if (want_x) {
     auto shape = dy.sizes().vec();
     shape.back() = w.size(-1);
-    dx = (plain_product(dy, w)
-              ? at::mm(dy3.view({-1, dy.size(-1)}), w)
-              : linear_grad_input_t(dy3, w.contiguous())).view(shape);
+    dx = linear_grad_input_t(dy3, w.contiguous()).view(shape);
   }
   if (want_w)
     dw = ungroup(linear_grad_weight_t(dy3, groups3(q, groups),

@@ -85,7 +85,7 @@ struct Params {
   // STORE
   void* out;
   long long out_ld, out_group;
-  int out_f32, accumulate;
+  int accumulate;
   const void* bias;
   long long bias_group;
   float* partial;
@@ -129,6 +129,7 @@ __device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&o)[3]) {
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 typedef u32x2 u32x2_u __attribute__((aligned(1)));
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 
 template <typename T>
 using Global = const __attribute__((address_space(1))) T*;
@@ -386,6 +387,12 @@ __device__ __forceinline__ void fold(float (&sum)[N], int o, int lane,
   if (up) lo += LEN;
 }
 
+// LDS written by other lanes of the wave before it can be read behind it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <Src S>
@@ -461,6 +468,10 @@ void gemm_kernel(Params p) {
     for (int q = 0; q < PA; ++q)
       fa[q] = LA::frag(ta + q * LA::PLANE, wm + u % MF * 32, u / MF);
   };
+  // bf16 outputs are computed transposed, with m along the lanes: a lane's
+  // values lie along a row and go to LDS, and from there to memory, 16 bytes
+  // at a time.
+  constexpr bool ACROSS = E == STORE && SA == BF16;
   auto products = [&](int u, const bf16x8 (&fa)[PA]) {
     const int i = u % MF;
     const bf16x8(&fb)[NF][PB] = fbs[u / MF & 1];
@@ -472,7 +483,8 @@ void gemm_kernel(Params p) {
 #pragma unroll
         for (int j = 0; j < NF; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              fa[qa], fb[j][qb], acc[i][j], 0, 0, 0);
+              ACROSS ? fb[j][qb] : fa[qa], ACROSS ? fa[qa] : fb[j][qb],
+              acc[i][j], 0, 0, 0);
       }
   };
   auto multiply = [&](const bf16* ta, const bf16* tb) {
@@ -605,7 +617,80 @@ void gemm_kernel(Params p) {
   const int m0 = tm * H::BM + wm, n0 = tn * H::BN + wn;
   const int M = p.a.rows, N = p.b.rows;
 
-  if constexpr (E == STORE) {
+  if constexpr (ACROSS) {
+    // Each wave passes 32 rows at a time through LDS of its own and writes
+    // them in whole lines (32768 x 1024 x 4096: 426 us with a 2-byte store a
+    // value, 287 so).
+    constexpr int W = NF * 32, LD = W + 4;        // LD: rows on other banks
+    constexpr int LANES = W / 8, HALF = H::WM * H::WN / 2;
+    static_assert(HALF * 32 * LD * 4 <= 2 * LA::PLANE * 2
+                  && HALF * 32 * LD * 4 <= 2 * LB::PLANE * 2);
+    __syncthreads();                              // the tiles have been read
+    float* stage = reinterpret_cast<float*>(wave < HALF ? sa[0] : sb[0])
+        + wave % HALF * (32 * LD);
+    const float scale = scale_of(p.scale, g);
+    const bool finite = fabsf(scale) < INFINITY;
+    const int c = lane % LANES * 8, n = n0 + c, left = N - n;
+    float bias[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      bias[t] = p.bias && !p.partial && t < left
+          ? bias_at<BF16>(p.bias, g * p.bias_group + n + t) : 0.f;
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(
+              stage + (lane & 31) * LD + j * 32 + acc_row(4 * q, lane)) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1],
+                    acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      wave_fence();
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += 64 / LANES) {
+        const int row = r0 + lane / LANES, m = m0 + i * 32 + row;
+        if (m >= M || left <= 0) continue;
+        float v[8];
+        load_n<8>(stage + row * LD + c, v);
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          v[t] = finite ? fmaf(v[t], scale, bias[t])
+                        : scaled(v[t], scale) + bias[t];
+        if (p.partial) {
+          float* o = p.partial
+              + (((long long)split * gridDim.z + g) * M + m) * N + n;
+          if (left >= 8) {
+#pragma unroll
+            for (int t = 0; t < 8; t += 4) {
+              f32x4 s = {v[t], v[t + 1], v[t + 2], v[t + 3]};
+              f32x4_u* at = reinterpret_cast<f32x4_u*>(o + t);
+              if (p.accumulate) s += *at;
+              *at = s;
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              if (t < left) o[t] = p.accumulate ? o[t] + v[t] : v[t];
+          }
+        } else {
+          bf16* o = static_cast<bf16*>(p.out) + g * p.out_group
+              + (long long)m * p.out_ld + n;
+          if (left >= 8) {
+            bf16x8 s;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) s[t] = (bf16)v[t];
+            *reinterpret_cast<bf16x8_u*>(o) = s;
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              if (t < left) o[t] = (bf16)v[t];
+          }
+        }
+      }
+      wave_fence();
+    }
+  } else if constexpr (E == STORE) {
     const float scale = scale_of(p.scale, g);
     const bool finite = fabsf(scale) < INFINITY;
 #pragma unroll
@@ -614,8 +699,7 @@ void gemm_kernel(Params p) {
       if (n >= N) continue;
       float bias = 0.f;
       if (p.bias && !p.partial)
-        bias = p.out_f32 ? bias_at<F32>(p.bias, g * p.bias_group + n)
-                         : bias_at<BF16>(p.bias, g * p.bias_group + n);
+        bias = bias_at<F32>(p.bias, g * p.bias_group + n);
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
 #pragma unroll
@@ -629,11 +713,8 @@ void gemm_kernel(Params p) {
                 + (((long long)split * gridDim.z + g) * M + m) * N + n;
             *o = p.accumulate ? *o + v : v;
           } else {
-            const long long at = g * p.out_group + (long long)m * p.out_ld + n;
-            if (p.out_f32)
-              static_cast<float*>(p.out)[at] = v;
-            else
-              static_cast<bf16*>(p.out)[at] = (bf16)v;
+            static_cast<float*>(p.out)[g * p.out_group
+                                       + (long long)m * p.out_ld + n] = v;
           }
         }
       }
@@ -1047,7 +1128,6 @@ void gemm(const Gemm& g, hipStream_t s) {
   p.out = g.out;
   p.out_ld = g.out_ld;
   p.out_group = g.out_group;
-  p.out_f32 = g.tout == kF32;
   p.accumulate = g.accumulate;
   p.bias = g.bias;
   p.bias_group = g.bias_group;

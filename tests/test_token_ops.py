@@ -1273,3 +1273,71 @@ def test_shared_weight_is_not_copied_per_client():
         out = torch.func.vmap(f)(x, b, y)
         assert torch.cuda.max_memory_allocated() - before < 100 << 20
         del out
+
+
+# ------------------------------------------- bf16 on the framework's kernels
+
+@gpu
+def test_bf16_products_are_the_operators_own():
+    """A product that the operators left to the library would take the type
+    that autocast gives the library's products."""
+    x, w = (rand(64, 48, dtype=torch.bfloat16, device="cuda", seed=i)
+            for i in range(2))
+    b = rand(64, dtype=torch.bfloat16, device="cuda")
+    f = torch.ops.blades_amd.linear_act8
+    g = torch.ops.blades_amd.linear_act8_grad
+    y, q, e, tie = f(x, w, b, True, 0)
+    dy = torch.ones_like(y)
+    want = (y, *g(dy, w, q, e, tie, 0, True, True, True))
+    with torch.autocast("cuda", torch.float16):
+        got = (f(x, w, b, True, 0)[0],
+               *g(dy, w, q, e, tie, 0, True, True, True))
+    for a, r in zip(got, want):
+        assert a.dtype == torch.bfloat16 and torch.equal(a, r)
+
+
+@gpu
+@pytest.mark.parametrize("fn", FNS)
+def test_bf16_results_repeat(fn):
+    w, b, x, y, up = population(fn, 6, "cuda", torch.bfloat16)
+    x = x.repeat(1, 200, 1)
+    y = y.repeat(1, 200)
+    if fn is not loss_fn:
+        up = up.repeat(1, 200, 1)
+    first = one_by_one(fn, w, b, x, y, up)
+    for _ in range(3):
+        for a, r in zip(one_by_one(fn, w, b, x, y, up), first):
+            assert torch.equal(a, r)
+
+
+@gpu
+def test_bf16_step_captured():
+    """Linear layer and loss of one client, captured and replayed on new
+    inputs with eager work between the replays."""
+    x = rand(700, 96, dtype=torch.bfloat16, device="cuda")
+    w = rand(96, 96, dtype=torch.bfloat16, device="cuda", seed=1)
+    v = rand(1000, 96, dtype=torch.bfloat16, device="cuda", seed=2)
+    y = torch.randint(0, 1000, (700,), device="cuda")
+
+    def step(x, w, v):
+        def loss(x, w, v):
+            return ops.linear_cross_entropy(ops.linear_act8(x, w), v, y)
+        grads, value = torch.func.grad_and_value(loss, argnums=(0, 1, 2))(
+            x, w, v)
+        return (value, *grads)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step(x, w, v)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, w, v)
+    for i in range(4):
+        x.copy_(rand(700, 96, dtype=torch.bfloat16, device="cuda", seed=9 + i))
+        graph.replay()
+        want = step(x, w, v)
+        torch.cuda.synchronize()
+        for a, r in zip(out, want):
+            assert torch.equal(a, r)
