@@ -19,6 +19,9 @@ and no gradient is taken per client at both levels; a loss that is summed or
 averaged per client needs the parameters shared at both.  Other nestings are
 refused.  The operators' gradients are not differentiable
 again.
+
+Under ``torch.autocast`` norms run in float32, products in bfloat16 where that
+is autocast's type, and in float32 where it is float16.
 """
 from __future__ import annotations
 
@@ -70,6 +73,29 @@ def _check_param(name: str, p: Optional[Tensor], x: Tensor, shape) -> None:
     if tuple(p.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got "
                          f"{tuple(p.shape)}")
+
+
+def _autocast(x, kind: str, *rest):
+    """``x`` and the parameters in the type that autocast runs the operator
+    in, as torch has it: ``"norm"`` in float32, ``"product"`` in autocast's
+    type, ``"any"`` in its input's.  float32 takes float16's place.  Outside
+    of autocast they stay as they are."""
+    device = x.device.type if isinstance(x, torch.Tensor) else ""
+    if device not in ("cpu", "cuda") or not torch.is_autocast_enabled(device):
+        return (x, *rest)
+    want = torch.float32
+    if kind == "any" and x.dtype != torch.float16:
+        want = x.dtype
+    elif kind == "product" and \
+            torch.get_autocast_dtype(device) == torch.bfloat16:
+        want = torch.bfloat16
+
+    def cast(t):
+        if isinstance(t, torch.Tensor) and t.dtype in (*_DTYPES,
+                                                       torch.float16):
+            return t.to(want)
+        return t
+    return tuple(cast(t) for t in (x, *rest))
 
 
 # ------------------------------------------------------------- vmap helpers
@@ -206,6 +232,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None,
     ``weight``, ``bias``: [dim] in x's type, or None.  Statistics and the
     sums of the gradients are 32-bit; each output is rounded once.
     """
+    x, weight, bias = _autocast(x, "norm", weight, bias)
     _check_input("x", x)
     _check_param("weight", weight, x, x.shape[-1:])
     _check_param("bias", bias, x, x.shape[-1:])
@@ -347,6 +374,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     stream: its row's loss, and every gradient it enters, is NaN.  ``bias``
     may hold -inf for words that are switched off.
     """
+    x, weight, bias = _autocast(x, "product", weight, bias)
     _check_input("x", x)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be a [vocab, dim] tensor")
@@ -428,6 +456,7 @@ def gelu_act8(x: Tensor) -> Tensor:
     holds an infinity or NaN has gradient NaN.  The output comes from ``x``
     itself.
     """
+    x, = _autocast(x, "any")
     _check_input("x", x)
     ext = _extension(x)
     if ext is not None:
@@ -556,6 +585,7 @@ def linear_act8(x: Tensor, weight: Tensor,
     In float32 a value that is not finite makes the results it enters NaN,
     and magnitudes below 2**-110 lose low bits.
     """
+    x, weight, bias = _autocast(x, "product", weight, bias)
     _check_input("x", x)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be an [out, in] tensor")

@@ -9,6 +9,7 @@ d model dims) unless noted.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -300,6 +301,16 @@ def gelu_backward(dy: Tensor, q: Tensor, e: Tensor) -> Tensor:
     return (dy.float() * slope).to(dy.dtype)
 
 
+def _full_precision(fn):
+    """Products in the types given to them, also under autocast."""
+    @functools.wraps(fn)
+    def run(x: Tensor, *args, **kw):
+        with torch.autocast(x.device.type, enabled=False):
+            return fn(x, *args, **kw)
+    return run
+
+
+@_full_precision
 def linear_forward(x: Tensor, w: Tensor, b: Optional[Tensor]) -> Tensor:
     y = torch.matmul(x.float(), w.float().transpose(-1, -2).contiguous())
     if b is not None:
@@ -307,10 +318,12 @@ def linear_forward(x: Tensor, w: Tensor, b: Optional[Tensor]) -> Tensor:
     return y.to(x.dtype)
 
 
+@_full_precision
 def linear_grad_input(dy: Tensor, w: Tensor) -> Tensor:
     return torch.matmul(dy.float(), w.float()).to(dy.dtype)
 
 
+@_full_precision
 def linear_grad_weight(dy: Tensor, q: Tensor, e: Tensor) -> Tensor:
     dyt = dy.float().transpose(1, 2).contiguous()
     return torch.matmul(dyt, act8_unpack(q, e)).to(dy.dtype)
@@ -321,6 +334,7 @@ def _logits(x: Tensor, w: Tensor, bias: Optional[Tensor]) -> Tensor:
     return z if bias is None else z + _per_row(bias)
 
 
+@_full_precision
 def loss_forward(x: Tensor, w: Tensor, target: Tensor,
                  bias: Optional[Tensor], ignore: int, reduction: int):
     """reduction 0: rows, 1: sum, 2: mean."""
@@ -342,6 +356,7 @@ def loss_forward(x: Tensor, w: Tensor, target: Tensor,
     return total.float(), lse, count
 
 
+@_full_precision
 def loss_backward(grad: Tensor, x: Tensor, w: Tensor, target: Tensor,
                   bias: Optional[Tensor], lse: Tensor, count: Tensor,
                   ignore: int, reduction: int, want_x: bool, want_w: bool,

@@ -104,6 +104,28 @@ def test_layers_pickled_without_the_choice_of_gelu(make):
     assert torch.equal(old(x), want)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("make", [text_model, image_model])
+def test_models_under_autocast(device, cast, make):
+    """The framework's layers where torch's run.  Both sides round at every
+    layer; each of a dozen steps moves an output by at most 2^-8 of the
+    largest value on its way, an order below the tolerance."""
+    torch.manual_seed(0)
+    plain = make().to(device)
+    own = make(fused_norm=True, act_bits=8).to(device)
+    own.load_state_dict(plain.state_dict())
+    x, y = batch(plain, device)
+    with torch.autocast(device, cast):
+        a = plain(x).float()
+        b = own(x).float()
+        loss = own(x, targets=y)
+    assert loss.dtype == torch.float32
+    assert (a - b).abs().max() <= 0.1 * a.abs().max()
+    for p, g in zip(own.parameters(), grads_of(loss, own)):
+        assert g.dtype == p.dtype and g.isfinite().all()
+
+
 class TokenDataset:
     """Next-word data of a few clients: (ids, the word to come)."""
 

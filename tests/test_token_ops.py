@@ -1341,3 +1341,57 @@ def test_bf16_step_captured():
         torch.cuda.synchronize()
         for a, r in zip(out, want):
             assert torch.equal(a, r)
+
+
+# ---------------------------------------------------------------- autocast
+
+CASTS = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cast", CASTS)
+def test_autocast_types(device, cast):
+    """Under autocast an operator is the one of inputs cast beforehand: norms
+    in float32, products in bfloat16, and float32 for float16."""
+    x, w, y, b = loss_inputs(9, 24, 24, torch.float32, device)
+    low = torch.bfloat16 if cast == torch.bfloat16 else torch.float32
+    calls = [(lambda x, w, b: ops.layer_norm(x, w[0], b), torch.float32),
+             (lambda x, w, b: ops.linear_act8(x, w, b), low),
+             (lambda x, w, b: ops.linear_cross_entropy(x, w, y, b), low)]
+    for f, typed in calls:
+        def run(*args):
+            out = f(*args)
+            return (out, *torch.autograd.grad(out.float().sum(), args))
+        # what a layer before this one may hand over, and parameters
+        for given in (torch.float32, cast):
+            leaves = [x.to(given), w.clone(), b.clone()]
+            for t in leaves:
+                t.requires_grad_()
+            with torch.autocast(device, cast):
+                got = run(*leaves)
+            want = run(*[t.detach().to(given if i == 0 else t.dtype).to(typed)
+                         .requires_grad_() for i, t in enumerate(leaves)])
+            assert got[0].dtype == want[0].dtype
+            assert torch.equal(got[0], want[0])
+            for a, r, t in zip(got[1:], want[1:], leaves):
+                assert a.dtype == t.dtype and torch.equal(a, r.to(a.dtype))
+    with torch.autocast(device, cast):
+        assert ops.gelu_act8(x).dtype == torch.float32
+        assert ops.gelu_act8(x.to(cast)).dtype == low
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autocast_around_forward_and_backward(device):
+    """torch.func's transforms run the backward pass inside autocast, too."""
+    w, b, x, y, up = population(gelu_linear_fn, 4, device)
+    low = [t.bfloat16() for t in (w, b, x)]
+
+    def step(w, b, x):
+        return torch.func.grad(lambda *a: gelu_linear_fn(*a, None).float()
+                               .sum(), argnums=(0, 1, 2))(w, b, x)
+    run = torch.func.vmap(step)
+    want = run(*low)
+    with torch.autocast(device, torch.bfloat16):
+        got = run(w, b, x)
+    for a, r in zip(got, want):
+        assert torch.equal(a, r.to(a.dtype))
