@@ -1,6 +1,7 @@
 // torch's vmap headers include nlohmann/json.hpp, which torch does not ship,
 // to write their interpreters out.  Nothing here does that: declarations are
-// enough, and a call would not link.
+// enough, and a call would not link.  Searched after every other include path,
+// so a header that is there goes before this one.
 #pragma once
 
 #include <string>

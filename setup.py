@@ -23,11 +23,12 @@ setup(
             sources=["csrc/blades_kernels.hip", "csrc/token_bindings.cpp",
                      "csrc/layer_norm.hip", "csrc/act8.hip",
                      "csrc/token_gemm.hip"],
-            include_dirs=[os.path.join(os.path.dirname(
-                os.path.abspath(__file__)), "csrc", "compat")],
             depends=["csrc/token_ops.h", "csrc/token_device.h"],
             extra_compile_args={
-                "cxx": ["-O3"],
+                # stands in only where no other path has such a header
+                "cxx": ["-O3", "-idirafter", os.path.join(
+                    os.path.dirname(os.path.abspath(__file__)), "csrc",
+                    "compat")],
                 # no packed fp32 instructions: some of their forms have
                 # given wrong results on this hardware
                 "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
