@@ -224,6 +224,9 @@ def norm_forward(x: Tensor, w: Optional[Tensor], b: Optional[Tensor],
     xf = x.float()
     mean = xf.mean(-1, keepdim=True)
     c = xf - mean
+    # the centred values' own mean: what the first sum rounded away
+    off = c.mean(-1, keepdim=True)
+    mean, c = mean + off, c - off
     rstd = 1.0 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
     y = c * rstd
     if w is not None:

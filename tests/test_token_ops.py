@@ -1395,3 +1395,18 @@ def test_autocast_around_forward_and_backward(device):
         got = run(w, b, x)
     for a, r in zip(got, want):
         assert torch.equal(a, r.to(a.dtype))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [256, 1000, 4096, 5001, 20001])
+def test_norm_mean_is_the_nearest(device, dim):
+    """Rows around 1000: the mean (512 to 1024) is off by its rounding to
+    fp32, half of 2^-14, and not by that of the sum of a thousand such values.
+    A tenth is left for the mean of the centred values; x - mean is exact and
+    the rest is 64 U of h: deviation, product and output."""
+    x = rand(64, dim, device=device, shift=1000.0)
+    y = ops.layer_norm(x).double()
+    xd = x.double()
+    c = xd - xd.mean(-1, keepdim=True)
+    r = 1 / (c.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    near(y, c * r, 1.1 * 2.0 ** -15 * r + 64 * U * (1 + (c * r).abs()))
