@@ -1271,6 +1271,15 @@ Tensor linear_cross_entropy_py(const Tensor& x, const Tensor& w,
   return std::get<0>(loss_op().call(x, w, target, b, ignore, reduction, 0));
 }
 
+std::tuple<int, int> product_tiling_py(int64_t groups, int64_t m, int64_t n,
+                                       int64_t k, bool deep, bool fp32,
+                                       bool act8) {
+  int tile, splits;
+  product_tiling(groups, m, n, k, deep, fp32 ? kF32 : kBF16, act8, &tile,
+                 &splits);
+  return {tile, splits};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(blades_amd, m) {
@@ -1333,6 +1342,8 @@ void bind_token_ops(pybind11::module_& m) {
   m.def("gelu_act8", &gelu_act8_py, nogil(), "GELU, its input kept in 8 bits");
   m.def("linear_act8", &linear_act8_py, nogil(),
         "linear layer, its input kept in 8 bits");
+  m.def("_product_tiling", &product_tiling_py,
+        "(tile rows, parts) of a product, for tests");
   m.def("linear_cross_entropy", &linear_cross_entropy_py, nogil(),
         "cross entropy of a linear head without its logits");
 }

@@ -1119,6 +1119,13 @@ int gemm_splits(const Gemm& g) {
                 products_of(g.ta, g.b.e != nullptr)).splits;
 }
 
+void product_tiling(long long groups, long long m, long long n, long long k,
+                    bool deep, DType a, bool b_act8, int* tile, int* splits) {
+  const Tiling t = tiling(groups, m, n, k, deep, products_of(a, b_act8));
+  *tile = kTileM[t.size];
+  *splits = t.splits;
+}
+
 void gemm(const Gemm& g, hipStream_t s) {
   Params p = {};
   p.a = make_op(g.a, g.a_kmajor, g.m, g.k);

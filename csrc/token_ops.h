@@ -29,7 +29,8 @@ struct NormArgs {
   float* rstd;
   void* dw;           // backward, may be null
   void* db;           // backward, may be null
-  float* partial;     // backward workspace, norm_partial_floats() floats
+  float* partial;     // backward workspace,
+                      // [groups][norm_partial_blocks()][2][dim]
   long long groups, rows, dim;
   long long w_stride, b_stride;  // elements between groups' parameters
   float eps;
@@ -101,6 +102,10 @@ struct Gemm {
 // Parts the contraction is best cut into (1: write `out` at once).
 int gemm_splits(const Gemm& g);
 void gemm(const Gemm& g, hipStream_t s);
+// Rows of the square output tile and parts of the contraction that a product
+// takes; `deep`: whether it may be cut.  For tests that have to reach each.
+void product_tiling(long long groups, long long m, long long n, long long k,
+                    bool deep, DType a, bool b_act8, int* tile, int* splits);
 // out = sum over splits of partial (+ bias), rounded to tout; a group's rows
 // lie without gaps
 void join_partials(const float* partial, int splits, long long groups,
