@@ -1410,3 +1410,51 @@ def test_norm_mean_is_the_nearest(device, dim):
     c = xd - xd.mean(-1, keepdim=True)
     r = 1 / (c.square().mean(-1, keepdim=True) + 1e-5).sqrt()
     near(y, c * r, 1.1 * 2.0 ** -15 * r + 64 * U * (1 + (c * r).abs()))
+
+
+# ------------------------------------------------------------------ memory
+
+def _peak(f):
+    """f's result, and the most that was allocated on the way beyond what was
+    before."""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = f()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_loss_memory(dtype):
+    """4096 x 50000 logits are 820 MB in fp32.  Forward: a maximum and a sum
+    per row and 64 words or more.  Backward: the gradients returned, 256 MiB
+    of logit gradient, 32-bit sums of dx, which may come in parts (at most
+    16 here), the join of db, and 16 MiB for what the rows need."""
+    rows, dim, vocab = 4096, 128, 50000
+    x = rand(rows, dim, dtype=dtype, device="cuda").requires_grad_()
+    w = rand(vocab, dim, dtype=dtype, device="cuda").requires_grad_()
+    b = rand(vocab, dtype=dtype, device="cuda").requires_grad_()
+    y = torch.randint(0, vocab, (rows,), device="cuda")
+    loss, peak = _peak(lambda: ops.linear_cross_entropy(x, w, y, b))
+    assert peak <= rows * (vocab // 64 + 1) * 8 + (1 << 20)
+    grads, peak = _peak(lambda: torch.autograd.grad(loss, (x, w, b)))
+    own = sum(g.numel() * g.element_size() for g in grads)
+    parts = 16 * rows * dim * 4
+    join = 4 * vocab * (rows // 32)
+    assert peak <= own + (256 << 20) + parts + join + (16 << 20)
+
+
+@gpu
+def test_act8_memory():
+    """Between forward and backward a chain linear, GELU, linear holds its
+    three inputs in 129/128 bytes a value (a block's exponent is one byte)."""
+    n, d = 1 << 15, 512
+    w = [rand(d, d, device="cuda", seed=i).requires_grad_() for i in range(2)]
+    x = rand(n, d, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = ops.linear_act8(ops.gelu_act8(ops.linear_act8(x, w[0])), w[1])
+    kept = torch.cuda.memory_allocated() - before
+    assert kept <= y.numel() * 4 + 3 * n * d * 129 // 128 + (1 << 20)
