@@ -15,8 +15,8 @@
 //
 // Bound by memory in fp32 (9 bytes a value each way) and close to the vector
 // units' rate in bf16 (5 bytes): Phi is built from one exp and a short
-// polynomial instead of the library's two-branch erf, which alone takes
-// longer than the bf16 traffic.  16 threads own a block of 128, 8 values
+// polynomial (in fp32 a second one near 0) instead of the library's two-branch
+// erf, which alone takes longer than the bf16 traffic.  16 threads own a block of 128, 8 values
 // each; the maximum crosses lanes by four shuffles.  Measured: 409600 x 512
 // bf16 forward 242 us, backward 243 us, 4.3 TB/s both; 32768 x 1024 packed in
 // 20 to 25 us.
@@ -65,7 +65,26 @@ __device__ __forceinline__ float normal_cdf(float x, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(TailC<T>::c, a, 1.f));
   e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);  // -log2(e)/2
   const float tail = e * (t * tail_q<T>(t));
-  return x < 0.f ? tail : 1.f - tail;
+  const float far = x < 0.f ? tail : 1.f - tail;
+  if constexpr (sizeof(T) == 4) {
+    // Near 0 the quotient's and the exponential's errors would show: there
+    // Phi = 1/2 + x S(x^2), the series of the density's integral, up to
+    // x^15 (2e-9 left at 1).  Relative error of x * Phi for |x| < 1 in half
+    // steps of fp32: 0.8 on average and 4 at most, where the quotient alone
+    // has 1.9 and 7.
+    const float s = a * a;
+    float q = -4.122667363e-8f;
+    q = fmaf(q, s, 6.659693668e-7f);
+    q = fmaf(q, s, -9.444655916e-6f);
+    q = fmaf(q, s, 1.1543469009e-4f);
+    q = fmaf(q, s, -1.1873282492e-3f);
+    q = fmaf(q, s, 9.973556735e-3f);
+    q = fmaf(q, s, -6.649038196e-2f);
+    q = fmaf(q, s, 0.3989422917f);
+    return a < 1.f ? fmaf(x, q, 0.5f) : far;
+  } else {
+    return far;
+  }
 }
 
 // Biased exponent of the block whose largest |x| has these bits; 255 where

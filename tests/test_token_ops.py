@@ -1458,3 +1458,17 @@ def test_act8_memory():
     y = ops.linear_act8(ops.gelu_act8(ops.linear_act8(x, w[0])), w[1])
     kept = torch.cuda.memory_allocated() - before
     assert kept <= y.numel() * 4 + 3 * n * d * 129 // 128 + (1 << 20)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lo,hi", [(-1.0, 0.0), (0.0, 1.0)])
+def test_gelu_rounding_near_zero(device, lo, hi):
+    """fp32 values up to 1, where most activations lie.  Roundings are even
+    within half a step, U / sqrt(3) each on average: of Phi, of the product,
+    and of the part of Phi beyond (or short of) 1/2, which a negative x
+    weighs by up to 2.1 and 0.7 on average: together 1.1 U or less."""
+    g = torch.Generator().manual_seed(0)
+    x = (torch.rand(300, 1024, generator=g) * (hi - lo) + lo).to(device)
+    want = gelu64(x)
+    err = ((ops.gelu_act8(x).double() - want) / want)[x != 0]
+    assert err.square().mean().sqrt() <= 1.25 * U
