@@ -359,7 +359,13 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     in float32, computed in tiles: the [rows, vocab] logits are never stored.
     The backward pass computes them again, a piece of the vocabulary at a
     time (at most 256 MiB of their gradient exists at once, or 512 words); it
-    takes fewer than 2**22 rows a client.
+    takes fewer than 2**22 rows a client, or of all clients together where
+    they share the parameters and the gradient is that of the whole vmap.
+
+    bfloat16 inputs are multiplied as they are and summed in float32.  The
+    logits' gradient is rounded to bfloat16 before the products that give
+    ``x``'s and ``weight``'s, which adds less than a hundredth to the error
+    that their own rounding has.
 
     ``x``: [..., dim]; ``weight``: [vocab, dim]; ``bias``: [vocab] or None;
     ``target``: int64, x's leading shape.  Rows whose target is
@@ -368,7 +374,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor,
     where none does, as torch has it; their gradient is zero).
 
     In float32 a value of ``x`` or ``weight`` that is not finite makes the
-    results it enters NaN.
+    results it enters NaN; in bfloat16 they are not finite.  An ignored row
+    enters the weight's gradient with a factor of zero, so it has to be finite
+    for that.
 
     A target outside the vocabulary cannot raise without stopping the GPU's
     stream: its row's loss, and every gradient it enters, is NaN.  ``bias``
@@ -454,7 +462,8 @@ def gelu_act8(x: Tensor) -> Tensor:
     which differ from ``x`` by at most ``2**(e-1)`` (what would round to
     2**128 is held as 63 * 2**122); a block of 128 that
     holds an infinity or NaN has gradient NaN.  The output comes from ``x``
-    itself.
+    itself; in float32 its relative error is about 2**-22 at most for ``|x| < 1``, and
+    grows with ``x**2`` in the negative tail.
     """
     x, = _autocast(x, "any")
     _check_input("x", x)
@@ -583,7 +592,8 @@ def linear_act8(x: Tensor, weight: Tensor,
     ``bias``: [out] or None.
 
     In float32 a value that is not finite makes the results it enters NaN,
-    and magnitudes below 2**-110 lose low bits.
+    and magnitudes below 2**-110 lose low bits.  ``in`` is below 2**22, and
+    for a gradient ``out`` too.
     """
     x, weight, bias = _autocast(x, "product", weight, bias)
     _check_input("x", x)

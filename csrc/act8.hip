@@ -18,8 +18,9 @@
 // polynomial (in fp32 a second one near 0) instead of the library's two-branch
 // erf, which alone takes longer than the bf16 traffic.  16 threads own a block of 128, 8 values
 // each; the maximum crosses lanes by four shuffles.  Measured: 409600 x 512
-// bf16 forward 242 us, backward 243 us, 4.3 TB/s both; 32768 x 1024 packed in
-// 20 to 25 us.
+// bf16 forward 237 us, backward 236 us, 4.4 TB/s both; 32768 x 1024 packed in
+// 20 to 25 us.  Rows that are not whole 16-byte accesses are read value by
+// value: 409600 x 509 bf16 forward 600 us, backward 571.
 
 #include "token_ops.h"
 #include "token_device.h"

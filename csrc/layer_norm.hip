@@ -15,7 +15,9 @@
 // without 16-byte alignment) take kernels that read the row again instead.
 // Measured: 16383 x 4096 bf16 forward 62 us (4.3 TB/s), backward 82 us
 // (4.9 TB/s, 7 us more to join); 204800 x 128 fp32 in 100 clients 37 and
-// 59 us.
+// 59 us.  One value an access costs: 16383 x 2047 bf16 67 and 61 us against 27
+// and 51 for 2048, 16383 x 4095 bf16, in the kernels that read again, 159 and
+// 248 against 54 and 92 (fp32: 273 and 342 against 98 and 161).
 
 #include "token_ops.h"
 #include "token_device.h"

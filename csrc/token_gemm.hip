@@ -26,11 +26,13 @@
 //   hands each lane 4 values down a column; 32-byte columns swizzled by k.
 // Sums are 32-bit in the accumulators.
 //
-// Bound by the matrix units: 46 to 62 percent busy in the long products (at
-// the clock such kernels run at, the library's bf16 product has 66), logits
-// 8192 x 50021 x 2048 bf16 in 1526 us, 1100 TFLOP/s; fp32 products of a few
-// hundred deep reach 150 to 170 TFLOP/s, about what the library's fp32 product
-// reaches at its best sizes.
+// Bound by the matrix units: 54 to 68 percent busy in the long bf16 products
+// (the library's have 63 to 75), 52 to 59 in fp32 ones of a few hundred deep
+// and many blocks, 25 to 45 where a block's few steps do not cover its start
+// and its output.  Logits 8192 x 50021 x 2048 bf16 in 1470 to 1520 us, 1100 to
+// 1140 TFLOP/s; fp32 logits 16 x 500 x 10000 x 300 in 290 to 316 us, 152 to
+// 166 TFLOP/s, and products with their gradient 118 to 130: about what the
+// library's fp32 product reaches at its best sizes (154).
 
 #include "token_ops.h"
 #include "token_device.h"
@@ -137,7 +139,7 @@ using Global = const __attribute__((address_space(1))) T*;
 // A pointer that is the same for all threads, held in scalar registers: left
 // to itself the compiler adds each thread's offset to it once and keeps the
 // sums, two registers a chunk, and spills (8-bit weight gradient 32768 x 4096
-// x 1024: 356 us so, 320 with the offsets alone; other products 1 to 4 %).
+// x 1024: 11 % slower so; other products 1 to 4 %).
 template <typename T>
 __device__ __forceinline__ Global<T> scalar(Global<T> p) {
   const uint64_t u = reinterpret_cast<uint64_t>(p);
@@ -403,7 +405,7 @@ __device__ __forceinline__ float bias_at(const void* p, long long i) {
 
 template <Src SA, bool KMA, Src SB, bool KMB, typename H, Epi E>
 // Small fp32 blocks are held to 168 registers so that three share a compute
-// unit: 211 -> 196 us for the two gradient products of 16 x 500 x 5000 x 300.
+// unit: 7 % less time for the two gradient products of 16 x 500 x 5000 x 300.
 __global__ __launch_bounds__(H::THREADS,
                              SrcOf<SA>::P == 3 && H::MF == 2 ? 3 : 1)
 void gemm_kernel(Params p) {
@@ -833,6 +835,12 @@ void gemm_kernel(Params p) {
           if (mr + 4 * (lane >> 5) == row) d -= 1.f;
           d = live && m0 + mr + 4 * (lane >> 5) < M ? d * ratio : 0.f;
           sum[i * 16 + r] += d;
+          // For bf16 inputs d goes to the two products in bf16: they take
+          // half the time and traffic that two bf16 parts of it would.  Its
+          // roundings (2^-8 of a term at most) are independent; the outputs'
+          // own rounding outweighs them: 8192 x 50021 x 2048, error against
+          // 64 bits 1.658e-3 for dx and 1.654e-3 for dw, where 32-bit terms
+          // rounded once have 1.655e-3 and 1.651e-3.
           if (SA == F32)
             static_cast<float*>(p.out)[at + mr * p.out_ld] = d;
           else
@@ -1054,10 +1062,9 @@ void launch(Params& p, long long groups, Size size, hipStream_t s) {
 // fp32) or three tiny at once.  A round's time is its area and its depth plus
 // a fixed part (filling the pipeline, the epilogue), which a large block alone
 // does not hide as well.  Measured: large tiles are 1.16 times as fast in the
-// long run (bf16 8192 x 50021 x 2048: 1580 against 1831 us), small ones win on
-// short contractions (fp32 16 x 500 x 5000 x 300: 170 against 187 us), tiny
-// ones where few blocks would leave units idle (fp32 2048 x 128 x 128: 8.7
-// against 19.7 us).
+// long run (bf16 logits 8192 x 50021 x 2048), small ones 1.1 times on short
+// contractions (fp32 logits 16 x 500 x 5000 x 300), tiny ones 2.3 times where
+// few blocks would leave units idle (fp32 2048 x 128 x 128, 8 us).
 struct Tiling {
   Size size;
   int splits;
