@@ -462,8 +462,8 @@ def gelu_act8(x: Tensor) -> Tensor:
     which differ from ``x`` by at most ``2**(e-1)`` (what would round to
     2**128 is held as 63 * 2**122); a block of 128 that
     holds an infinity or NaN has gradient NaN.  The output comes from ``x``
-    itself; in float32 its relative error is about 2**-22 at most for ``|x| < 1``, and
-    grows with ``x**2`` in the negative tail.
+    itself; in float32 its relative error is about 2**-22 at most for
+    ``|x| < 1`` and grows with ``x**2`` in the negative tail.
     """
     x, = _autocast(x, "any")
     _check_input("x", x)

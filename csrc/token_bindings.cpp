@@ -777,7 +777,8 @@ OptTensor or_none(const Tensor& t) {
   return t.defined() ? OptTensor(t) : OptTensor();
 }
 
-// Base of the nodes: tensors to keep, released together.
+// Base of the nodes: tensors to keep, released together.  A saved tensor may be
+// asked for once in a backward pass (checkpoints that recompute hold to it).
 struct TokenNode : public Node {
   std::vector<SavedVariable> saved;
   void keep(std::initializer_list<Tensor> ts) {
@@ -836,16 +837,15 @@ struct LinearNode : public TokenNode {          // w, q, e, tie
     const bool want[3] = {task_should_compute_output(0),
                           task_should_compute_output(1),
                           task_should_compute_output(2)};
+    const Tensor w = get(0), q = get(1), e = get(2), tie = get(3);
     // a shared weight's gradient is one product over all clients' rows
     const bool apart = shared_w && !shared_b && want[2];
     auto [dx, dw, db] =
-        linear_grad_op().call(grads[0], get(0), get(1), get(2), get(3),
-                              shared_w ? 0 : groups, want[0], want[1],
-                              want[2] && !apart);
+        linear_grad_op().call(grads[0], w, q, e, tie, shared_w ? 0 : groups,
+                              want[0], want[1], want[2] && !apart);
     if (apart)
-      db = std::get<2>(linear_grad_op().call(grads[0], get(0), get(1), get(2),
-                                             get(3), groups, false, false,
-                                             true));
+      db = std::get<2>(linear_grad_op().call(grads[0], w, q, e, tie, groups,
+                                             false, false, true));
     return {want[0] ? dx : Tensor(), want[1] ? dw : Tensor(),
             want[2] ? summed(db, shared_b && !shared_w) : Tensor()};
   }
@@ -861,9 +861,10 @@ struct LossNode : public TokenNode {            // x, w, target, b, lse, count
     const bool want[3] = {task_should_compute_output(0),
                           task_should_compute_output(1),
                           task_should_compute_output(2)};
-    Tensor grad = grads[0], w = get(1), target = get(2), count = get(5);
+    Tensor grad = grads[0], w = get(1), target = get(2), b = get(3),
+           count = get(5);
     int64_t red = reduction, g = groups;
-    const bool own_b = g && !shared_b && get(3).defined();
+    const bool own_b = g && !shared_b && b.defined();
     if (shared_w && !own_b) {
       // shared parameters: one sum over all clients' rows, each row with its
       // client's share of the upstream gradient
@@ -878,7 +879,7 @@ struct LossNode : public TokenNode {            // x, w, target, b, lse, count
       count = count.narrow(0, 0, 1);
     }
     auto [dx, dw, db] =
-        loss_grad_op().call(grad, get(0), w, target, or_none(get(3)), get(4),
+        loss_grad_op().call(grad, get(0), w, target, or_none(b), get(4),
                             count, ignore, red, g, want[0], want[1], want[2]);
     return {want[0] ? dx : Tensor(),
             want[1] ? summed(dw, g && shared_w) : Tensor(),

@@ -1472,3 +1472,33 @@ def test_gelu_rounding_near_zero(device, lo, hi):
     want = gelu64(x)
     err = ((ops.gelu_act8(x).double() - want) / want)[x != 0]
     assert err.square().mean().sqrt() <= 1.25 * U
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fn", FNS)
+@pytest.mark.parametrize("dims", [(None, None), (0, 0), (None, 0), (0, None)])
+def test_checkpointed(device, fn, dims):
+    """Recomputed in the backward pass, where each saved tensor may be asked
+    for once."""
+    from torch.utils.checkpoint import checkpoint
+    w, b, x, y, up = population(fn, 3, device)
+    if dims[0] is None:
+        w = w[0]
+    if dims[1] is None:
+        b = b[0]
+    leaves = [t.detach().clone().requires_grad_() for t in (w, b, x)]
+
+    def run(w, b, x):
+        return torch.func.vmap(fn, in_dims=dims + (0, 0))(w, b, x, y)
+    want = torch.autograd.grad(run(*leaves), leaves, up)
+    out = checkpoint(run, *leaves, use_reentrant=False)
+    for g, r in zip(torch.autograd.grad(out, leaves, up), want):
+        assert torch.equal(g, r)
+    one = [t[0] if d == 0 else t for t, d in zip(leaves, dims + (0,))]
+
+    def single(w, b, x):
+        return fn(w, b, x, y[0])
+    want = torch.autograd.grad(single(*one), leaves, up[0])
+    out = checkpoint(single, *one, use_reentrant=False)
+    for g, r in zip(torch.autograd.grad(out, leaves, up[0]), want):
+        assert torch.equal(g, r)
