@@ -255,7 +255,8 @@ class _HeadLossGrad(_NoSecond):
             _groups2(grad.float(), groups), _groups3(x, groups),
             w.contiguous(), _groups2(target, groups),
             None if b is None else b.contiguous(),
-            _groups2(lse, groups), count.reshape(g).contiguous(),
+            lse.reshape(g, lse.numel() // (2 * g), 2).contiguous(),
+            count.reshape(g).contiguous(),
             ignore, reduction, *wants)
         if not groups:
             dw = dw[0] if wants[1] else dw
@@ -294,7 +295,7 @@ class _HeadLoss(Function):
             loss = loss.view(target.shape)
         elif not groups:
             loss = loss[0]
-        return (loss, lse.view(target.shape),
+        return (loss, lse.view(*target.shape, 2),
                 count if groups else count[0])
 
     @staticmethod

@@ -340,16 +340,20 @@ def _logits(x: Tensor, w: Tensor, bias: Optional[Tensor]) -> Tensor:
 @_full_precision
 def loss_forward(x: Tensor, w: Tensor, target: Tensor,
                  bias: Optional[Tensor], ignore: int, reduction: int):
-    """reduction 0: rows, 1: sum, 2: mean."""
+    """reduction 0: rows, 1: sum, 2: mean.  The second output is [..., 2]: a
+    row's largest logit and the logarithm of its sum relative to that, whose
+    sum would round the logarithm away where logits are large."""
     vocab = w.shape[-2]
     z = _logits(x, w, bias)
-    lse = torch.logsumexp(z, -1)
+    top = z.amax(-1)
+    log = torch.log(torch.exp(z - top.unsqueeze(-1)).sum(-1))
     counted = target != ignore
     bad = counted & ((target < 0) | (target >= vocab))
-    lse = lse.masked_fill(bad, float("nan"))
+    top = top.masked_fill(bad, float("nan"))
+    lse = torch.stack([top, log], -1)
     at = target.clamp(0, vocab - 1).unsqueeze(-1)
-    rows = torch.where(counted, lse - z.gather(-1, at).squeeze(-1),
-                       torch.zeros_like(lse))
+    rows = torch.where(counted, (top - z.gather(-1, at).squeeze(-1)) + log,
+                       torch.zeros_like(top))
     count = counted.sum(-1).float()
     if reduction == 0:
         return rows, lse, count
@@ -365,7 +369,7 @@ def loss_backward(grad: Tensor, x: Tensor, w: Tensor, target: Tensor,
                   ignore: int, reduction: int, want_x: bool, want_w: bool,
                   want_b: bool):
     z = _logits(x, w, bias)
-    p = torch.exp(z - lse.unsqueeze(-1))
+    p = torch.exp((z - lse[..., :1]) - lse[..., 1:])
     counted = (target != ignore).unsqueeze(-1)
     at = target.clamp(0, w.shape[-2] - 1).unsqueeze(-1)
     p.scatter_add_(-1, at, torch.full_like(at, -1.0, dtype=p.dtype))

@@ -430,14 +430,14 @@ Loss loss_args(const Tensor& x, const Tensor& w, const Tensor& target,
 }
 
 // reduction 0: none, 1: sum, 2: mean.
-// -> loss ([groups] or [groups, rows]), lse [groups, rows], count [groups]
+// -> loss ([groups] or [groups, rows]), lse [groups, rows, 2], count [groups]
 std::tuple<Tensor, Tensor, Tensor> loss_forward_t(
     const Tensor& x, const Tensor& w, const Tensor& target,
     const OptTensor& bias, int64_t ignore, int64_t reduction) {
   Loss l = loss_args(x, w, target, bias, ignore);
   c10::DeviceGuard guard(x.device());
-  Tensor lse = floats(x, {l.groups, l.rows});
-  Tensor rows = at::empty_like(lse);
+  Tensor lse = floats(x, {l.groups, l.rows, 2});
+  Tensor rows = floats(x, {l.groups, l.rows});
   Tensor count = floats(x, {l.groups});
   if (l.rows == 0) {
     count.zero_();
@@ -450,7 +450,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_forward_t(
   loss_tile(l, &tile_m, &tile_n);
   Tensor part =
       floats(x, {l.groups, ceil_div(l.vocab, tile_m), l.rows, 2});
-  Tensor picked = at::empty_like(lse);
+  Tensor picked = at::empty_like(rows);
   Tensor loss, sums;
   if (reduction != 0) {
     loss = floats(x, {l.groups});
@@ -458,7 +458,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_forward_t(
                      x.options().dtype(at::kDouble));
   }
   loss_forward(l, part.data_ptr(), picked.data_ptr<float>(),
-               lse.data_ptr<float>(), rows.data_ptr<float>(),
+               lse.data_ptr(), rows.data_ptr<float>(),
                reduction ? sums.data_ptr() : nullptr,
                reduction ? loss.data_ptr<float>() : nullptr,
                count.data_ptr<float>(), reduction == 2, stream_of(x));
@@ -480,7 +480,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
   TORCH_CHECK(grad.scalar_type() == at::kFloat
               && lse.scalar_type() == at::kFloat
               && count.scalar_type() == at::kFloat
-              && lse.numel() == l.groups * l.rows
+              && lse.numel() == 2 * l.groups * l.rows
               && count.numel() == l.groups
               && grad.numel() == (reduction ? l.groups : l.groups * l.rows),
               "bad saved tensors");
@@ -543,7 +543,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward_t(
 
   for (long long v0 = 0; v0 < l.vocab; v0 += piece) {
     const long long nv = std::min(piece, l.vocab - v0);
-    loss_logit_grad(l, v0, nv, lse.data_ptr<float>(),
+    loss_logit_grad(l, v0, nv, lse.data_ptr(),
                     reduction ? nullptr : ratio.data_ptr<float>(),
                     pt.data_ptr(), ld, piece * ld,
                     want_b ? bsum.data_ptr<float>() : nullptr, s);
@@ -751,7 +751,9 @@ Int3 loss_cuda(const Tensor& x, const Tensor& w, const Tensor& target,
     loss = loss.view(target.sizes());
   else
     loss = ungroup(loss, groups, true);
-  return {loss, lse.view(target.sizes()), ungroup(count, groups, true)};
+  auto pairs = target.sizes().vec();
+  pairs.push_back(2);
+  return {loss, lse.view(pairs), ungroup(count, groups, true)};
 }
 
 Int3 loss_grad_cuda(const Tensor& grad, const Tensor& x, const Tensor& w,

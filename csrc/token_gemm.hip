@@ -96,7 +96,7 @@ struct Params {
   long long ignore, v0;
   float2* part;
   float* picked;
-  const float* lse;
+  const float2* lse;      // a row's maximum, and its sum's logarithm from there
   const float* ratio;     // [groups][n], null: all ones
   float* rowsum;          // [groups][tiles_n * WN][m], may be null
   Scale scale;            // of what STORE writes
@@ -813,13 +813,15 @@ void gemm_kernel(Params p) {
     for (int j = 0; j < NF; ++j) {
       const int n = n0 + j * 32 + (lane & 31);
       long long tgt = p.ignore;
-      float lse = 0.f, ratio = 1.f;
+      float2 lse = {0.f, 0.f};
+      float ratio = 1.f;
       if (n < N) {
         tgt = p.target[g * N + n];
         lse = p.lse[g * N + n];
         if (p.ratio) ratio = p.ratio[g * N + n];
       }
       const bool live = n < N && tgt != p.ignore;
+      const float less = lse.y * -kLog2e;
       const long long place = tgt - p.v0 - m0;
       const int row = place >= 0 && place < MF * 32 ? (int)place : -1;
       // whole tiles are written: readers need no bounds
@@ -831,7 +833,8 @@ void gemm_kernel(Params p) {
         for (int r = 0; r < 16; ++r) {
           const int mr = i * 32 + (r & 3) + 8 * (r >> 2);
           // beyond the vocabulary the logit is -inf: exp gives 0
-          float d = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e);
+          float d = __builtin_amdgcn_exp2f(
+              fmaf(acc[i][j][r] - lse.x, kLog2e, less));
           if (mr + 4 * (lane >> 5) == row) d -= 1.f;
           d = live && m0 + mr + 4 * (lane >> 5) < M ? d * ratio : 0.f;
           sum[i * 16 + r] += d;
@@ -914,7 +917,7 @@ void lse_kernel(const float2* __restrict__ part,
                 const float* __restrict__ picked,
                 const long long* __restrict__ target, long long ignore,
                 long long vocab, int tiles, long long rows,
-                float* __restrict__ lse, float* __restrict__ row_loss,
+                float2* __restrict__ lse, float* __restrict__ row_loss,
                 double2* __restrict__ sums) {
   constexpr int SEGS = kThreads / R;
   __shared__ float2 seg[SEGS][R];
@@ -949,15 +952,16 @@ void lse_kernel(const float2* __restrict__ part,
           mx = m;
         }
         const long long tgt = target[g * rows + n];
-        float l = mx + logf(sum);
+        const float l = logf(sum);
         float row = 0.f;
         if (tgt != ignore) {
-          if (tgt < 0 || tgt >= vocab) l = NAN;   // no such word
-          row = l - ((tgt < 0 || tgt >= vocab) ? 0.f : picked[g * rows + n]);
+          const bool word = tgt >= 0 && tgt < vocab;
+          if (!word) mx = NAN;
+          row = (mx - (word ? picked[g * rows + n] : 0.f)) + l;
           loss = row;
           cnt = 1.0;
         }
-        lse[g * rows + n] = l;
+        lse[g * rows + n] = make_float2(mx, l);
         row_loss[g * rows + n] = row;
       }
 #pragma unroll
@@ -1223,7 +1227,7 @@ Params loss_params(const Loss& l, long long v0, long long nv) {
 }
 }  // namespace
 
-void loss_forward(const Loss& l, void* part, float* picked, float* lse,
+void loss_forward(const Loss& l, void* part, float* picked, void* lse,
                   float* row_loss, void* block_sums, float* loss,
                   float* count, bool mean, hipStream_t s) {
   Params p = loss_params(l, 0, l.vocab);
@@ -1235,20 +1239,20 @@ void loss_forward(const Loss& l, void* part, float* picked, float* lse,
   const long long blocks = loss_sum_blocks(l.rows);
   const auto merge = lse_rows(l.rows) == 8 ? lse_kernel<8> : lse_kernel<32>;
   merge<<<dim3(grid_of(blocks), (unsigned)l.groups), kThreads, 0, s>>>(
-      p.part, picked, l.target, l.ignore, l.vocab, p.tiles_m, l.rows, lse,
-      row_loss, static_cast<double2*>(block_sums));
+      p.part, picked, l.target, l.ignore, l.vocab, p.tiles_m, l.rows,
+      static_cast<float2*>(lse), row_loss, static_cast<double2*>(block_sums));
   if (loss)
     loss_sum_kernel<<<dim3((unsigned)l.groups), kThreads, 0, s>>>(
         static_cast<const double2*>(block_sums), blocks, loss, count, mean);
 }
 
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
-                     const float* lse, const float* ratio, void* pt,
+                     const void* lse, const float* ratio, void* pt,
                      long long pt_ld, long long pt_group, float* rowsum,
                      hipStream_t s) {
   Params p = loss_params(l, v0, nv);
   p.rowsum = rowsum;
-  p.lse = lse;
+  p.lse = static_cast<const float2*>(lse);
   p.ratio = ratio;
   p.out = pt;
   p.out_ld = pt_ld;

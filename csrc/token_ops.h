@@ -126,11 +126,13 @@ struct Loss {
 // Tiles the loss is computed in: m words by n rows.
 void loss_tile(const Loss& l, int* m, int* n);
 // part: [groups][vocabulary tiles][rows] float2; picked: [groups][rows] float.
-// Writes lse and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
+// Writes lse, a row's largest logit and the logarithm of its sum relative to
+// that as float2 [groups][rows] (their sum would round the logarithm away where
+// logits are large), and row_loss [groups][rows]; with `loss` set also its sum (or mean) per
 // group and the number of counted rows, through block_sums
 // [groups][loss_sum_blocks(rows)] double2.
 long long loss_sum_blocks(long long rows);
-void loss_forward(const Loss& l, void* part, float* picked, float* lse,
+void loss_forward(const Loss& l, void* part, float* picked, void* lse,
                   float* row_loss, void* block_sums, float* loss,
                   float* count, bool mean, hipStream_t s);
 // Upstream gradients per row as top[g] * ratio[g][row], |ratio| <= 1.
@@ -143,7 +145,7 @@ void row_scale(const float* grad, long long groups, long long rows,
 // rowsum (may be null): [groups][loss_row_parts()][nv] sums over rows, before
 // any rounding to bf16.
 void loss_logit_grad(const Loss& l, long long v0, long long nv,
-                     const float* lse, const float* ratio, void* pt,
+                     const void* lse, const float* ratio, void* pt,
                      long long pt_ld, long long pt_group, float* rowsum,
                      hipStream_t s);
 long long loss_row_parts(const Loss& l);

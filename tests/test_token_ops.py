@@ -1502,3 +1502,72 @@ def test_checkpointed(device, fn, dims):
     out = checkpoint(single, *one, use_reentrant=False)
     for g, r in zip(torch.autograd.grad(out, leaves, up[0]), want):
         assert torch.equal(g, r)
+
+
+# --------------------------------------------- logits far from zero, masks
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_loss_masked_by_the_lowest_value(device, dtype):
+    """Words masked by the type's lowest value are switched off; where that
+    leaves none, all are alike, their softmax 1 / vocab."""
+    x, w, y, b = loss_inputs(20, 32, 300, dtype, device)
+    low = torch.finfo(dtype).min
+    off = b.clone()
+    off[5:] = -math.inf
+    masked = b.clone()
+    masked[5:] = low
+    y = torch.where(y == -100, y, y % 5)
+    got, want = (
+        (out, *torch.autograd.grad(out, leaves)) for out, leaves in (
+            (ops.linear_cross_entropy(*leaves[:2], y, leaves[2]), leaves)
+            for leaves in ([t.clone().requires_grad_() for t in (x, w, c)]
+                           for c in (masked, off))))
+    for a, r in zip(got, want):
+        assert torch.equal(a, r)
+    every = torch.full_like(b, low)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    rows = ops.linear_cross_entropy(*leaves, y, every, reduction="none")
+    keep = y != -100
+    # logarithm, sum of 300 ones and the last rounding
+    near(rows, torch.where(keep, math.log(300.0), 0.0), 32 * U)
+    dx, dw = torch.autograd.grad(rows.sum(), leaves)
+    p = torch.full((20, 300), 1 / 300, dtype=torch.float64, device=device)
+    p[torch.arange(20), y.clamp(min=0)] -= 1
+    p = torch.where(keep[:, None], p, torch.zeros_like(p))
+    # a term: its softmax's 32 U and its rounding; sums of 300 and 20 terms
+    k = (HALF[dtype] * 1.01 if dtype == torch.bfloat16 else 0) + 350 * U
+    for a, r, e in ((dx, p @ w.double(), p.abs() @ w.double().abs()),
+                    (dw, p.t() @ x.double(), p.abs().t() @ x.double().abs())):
+        near(a, r, HALF[dtype] * 1.01 * r.abs() + k * e)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loss_common_offset_of_the_logits(device):
+    """Whole-number logits around 2^20, exact in fp32: what they share costs
+    neither the loss nor the softmax any bits.  A loss has 8 U for its
+    exponentials and logarithm, U for each of 300 additions at most, and the
+    rounding of at most 40; a softmax those and its exponent's, 40 U more."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.ones(30, 16)
+    w = torch.randint(-1, 2, (300, 16), generator=g).float()
+    y = torch.randint(0, 300, (30,), generator=g)
+    b = torch.full((300,), 2.0 ** 20)
+    x, w, y, b = (t.to(device) for t in (x, w, y, b))
+    want, lse, z = loss64(x, w, y, b, -100)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    rows = ops.linear_cross_entropy(*leaves[:2], y, leaves[2],
+                                    reduction="none")
+    near(rows, want, 350 * U)
+    up = rand(30, device=device, seed=4)
+    dx, dw, db, p = loss_grads64(x, w, y, b, -100, up.double())
+    soft = torch.exp(z - lse[:, None]) * up.double().abs()[:, None]
+    ep = 400 * U * soft + 8 * U * p.abs()
+    got = torch.autograd.grad(rows, leaves, up)
+    for a, r, e in zip(got, (dx, dw, db),
+                       (ep @ w.double().abs() + 308 * U * (p.abs()
+                                                           @ w.double().abs()),
+                        ep.t() @ x.double() + 38 * U * (p.abs().t()
+                                                        @ x.double()),
+                        ep.sum(0) + 38 * U * p.abs().sum(0))):
+        near(a, r, e + 2 * U * r.abs())
