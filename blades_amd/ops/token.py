@@ -593,8 +593,9 @@ def linear_act8(x: Tensor, weight: Tensor,
     ``bias``: [out] or None.
 
     In float32 a value that is not finite makes the results it enters NaN,
-    and magnitudes below 2**-110 lose low bits.  ``in`` is below 2**22, and
-    for a gradient ``out`` too.
+    and magnitudes below 2**-110 lose low bits.  One in ``x`` makes the
+    weight's gradient NaN in all the columns of its block of 128, in either
+    type.  ``in`` is below 2**22, and for a gradient ``out`` too.
     """
     x, weight, bias = _autocast(x, "product", weight, bias)
     _check_input("x", x)

@@ -1571,3 +1571,61 @@ def test_loss_common_offset_of_the_logits(device):
                                                         @ x.double()),
                         ep.sum(0) + 38 * U * p.abs().sum(0))):
         near(a, r, e + 2 * U * r.abs())
+
+
+# ------------------------------------------------ offsets beyond 32 bits
+
+@gpu
+@pytest.mark.parametrize("fn", ["norm", "gelu", "linear", "loss"])
+def test_more_than_2_31_values(fn):
+    """The last rows of inputs of more than 2**31 values, forward and
+    gradient, against the same rows alone."""
+    dtype = torch.bfloat16
+    dim, last = 1032, 40
+    rows = (1 << 31) // dim + 100
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(rows, dim, dtype=dtype, device="cuda")
+    for lo in range(0, rows, 1 << 18):
+        hi = min(rows, lo + (1 << 18))
+        x[lo:hi] = torch.randn(hi - lo, dim, generator=g, device="cuda")
+    w = rand(24, dim, dtype=dtype, device="cuda", scale=dim ** -0.5)
+    b = rand(24, dtype=dtype, device="cuda")
+    y = torch.randint(0, 24, (rows,), generator=g, device="cuda")
+    f = {"norm": lambda x, y: ops.layer_norm(x, w[0], w[1]),
+         "gelu": lambda x, y: ops.gelu_act8(x),
+         "linear": lambda x, y: ops.linear_act8(x, w, b),
+         "loss": lambda x, y: ops.linear_cross_entropy(
+             x, w, y, b, reduction="none")}[fn]
+
+    def run(x, y):
+        x = x.requires_grad_()
+        out = f(x, y)
+        return out[-last:], torch.autograd.grad(
+            out, x, torch.ones((), dtype=out.dtype,
+                               device="cuda").expand_as(out))[0][-last:]
+    want = run(x[-last:].clone(), y[-last:])
+    got = run(x, y)
+    for a, r in zip(got, want):
+        close(a.float(), r.float(), torch.float32 if fn in ("norm", "gelu")
+              else dtype)
+
+
+@gpu
+def test_parameter_gradients_of_more_than_2_31_values():
+    """Per-client gradients of 24 heads, 2.4e9 values, in the last client."""
+    C, v, d = 24, 50000, 2048
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(C, 40, d, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(v, d, generator=g, device="cuda")
+         * d ** -0.5).bfloat16()
+    y = torch.randint(0, v, (C, 40), generator=g, device="cuda")
+
+    def step(x, y):
+        return torch.func.grad(
+            lambda x, w: ops.linear_cross_entropy(x, w, y),
+            argnums=(0, 1))(x, w)
+    got = torch.func.vmap(step)(x, y)
+    assert got[1].numel() > 1 << 31
+    for c in (0, C - 1):
+        for a, r in zip(got, step(x[c], y[c])):
+            close(a[c].float(), r.float(), torch.bfloat16)
