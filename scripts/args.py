@@ -14,6 +14,10 @@ import os
 import torch
 
 
+# models that take fused_norm and act_bits
+TRANSFORMERS = ("cct", "cct_2_3x2_32", "cvt", "vit_lite")
+
+
 def parse_arguments(argv=None):
     parser = argparse.ArgumentParser()
     parser.add_argument("--use-cuda", action="store_true", default=False)
@@ -44,6 +48,7 @@ def parse_arguments(argv=None):
     parser.add_argument("--fused_norm", action="store_true", default=False,
                         help="cct: layer norms on the framework's kernels")
     parser.add_argument("--act_bits", type=int, default=32,
+                        choices=[8, 32],
                         help="cct: bits of the activations kept for the "
                              "backward pass, 32 or 8")
     parser.add_argument("--engine", type=str, default="auto",
@@ -56,6 +61,11 @@ def parse_arguments(argv=None):
     parser.add_argument("--validate_interval", type=int, default=1)
     parser.add_argument("--data_root", type=str, default="./data")
     options = parser.parse_args(argv)
+    options.transformer = options.model.lower() in TRANSFORMERS
+    if not options.transformer and (options.fused_norm
+                                    or options.act_bits != 32):
+        parser.error("--fused_norm and --act_bits are for the transformers: "
+                     + ", ".join(TRANSFORMERS))
 
     ROOT_DIR = os.path.dirname(os.path.abspath(__file__))
     EXP_DIR = os.path.join(ROOT_DIR, f"outputs/{options.dataset}")

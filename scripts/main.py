@@ -59,7 +59,7 @@ def main():
         model_kw["norm"] = "batch-local"
     if options.dataset == "cifar100":
         model_kw["num_classes"] = 100
-    if options.model in ("cct", "cct_2_3x2_32", "cvt", "vit_lite"):
+    if options.transformer:
         model_kw.update(fused_norm=options.fused_norm,
                         act_bits=options.act_bits)
     model = get_model(options.model, **model_kw)

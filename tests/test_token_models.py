@@ -257,3 +257,22 @@ def test_operators_together(device, dtype):
         for a, r in zip(grads, want):
             a = a[c].double().cpu()
             assert (a - r).norm() <= 0.05 * r.norm()
+
+
+@pytest.mark.parametrize("argv,fine", [
+    (["--model", "cct", "--act_bits", "8", "--fused_norm"], True),
+    (["--model", "CCT", "--act_bits", "8"], True),
+    (["--model", "mlp"], True),
+    (["--model", "mlp", "--act_bits", "8"], False),
+    (["--model", "resnet18", "--fused_norm"], False),
+    (["--model", "cct", "--act_bits", "4"], False)])
+def test_command_line_options_are_not_dropped(monkeypatch, argv, fine):
+    """The transformers' options reach the model, and raise for others."""
+    monkeypatch.syspath_prepend("scripts")
+    from args import parse_arguments
+    if fine:
+        options = parse_arguments(argv)
+        assert options.transformer == (options.model.lower() == "cct")
+    else:
+        with pytest.raises(SystemExit):
+            parse_arguments(argv)
