@@ -106,7 +106,7 @@ class FusedEngine:
         g = grad(self._loss, argnums=0)
         return vmap(g, in_dims=((param_in,) * len(self.spec.names) if not shared_params else None,
                                 0, 0, 0, 0),
-                    chunk_size=self.client_chunk)
+                    chunk_size=self.client_chunk, randomness="different")
 
     # -------------------------------------------------------------- training
     base_loss = staticmethod(nn.functional.cross_entropy)

@@ -276,3 +276,69 @@ def test_command_line_options_are_not_dropped(monkeypatch, argv, fine):
     else:
         with pytest.raises(SystemExit):
             parse_arguments(argv)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kw", [{}, {"fused_norm": True, "act_bits": 8}])
+@pytest.mark.parametrize("make", [text_cct_2, CCT])
+def test_dropout_in_a_population(device, kw, make):
+    """The models as they come, with dropout and stochastic depth: clients of
+    the same data and parameters train as one batch and draw masks of their
+    own."""
+    from blades_amd.engine import FusedEngine, ParamSpec
+    torch.manual_seed(0)
+    if make is CCT:
+        model = CCT(img_size=16, embedding_dim=32, dropout=0.2, **kw)
+        x, y = torch.randn(1, 6, 3, 16, 16), torch.randint(0, 10, (1, 6))
+    else:
+        model = text_cct_2(seq_len=12, vocab_size=60, num_classes=60,
+                           word_embedding_dim=24, dropout=0.2, **kw)
+        x, y = torch.randint(1, 60, (1, 6, 12)), torch.randint(0, 60, (1, 6))
+    model = model.to(device).train()
+    engine = FusedEngine(model, ParamSpec.from_module(model), device,
+                         head_loss=True)
+    p = tuple(t.detach() for t in model.parameters())
+    x, y = (t.expand(4, *t.shape[1:]).to(device) for t in (x, y))
+    one = torch.ones(4, device=device)
+    for shared in (True, False):
+        args = p if shared else tuple(t.expand(4, *t.shape) for t in p)
+        grads = engine._build_grad_fn(shared)(args, x, y, one * 1e6, one)
+        head = grads[-1]
+        assert head.isfinite().all()
+        assert not torch.equal(head[0], head[1])
+
+
+@pytest.mark.gpu
+def test_captured_dropout_draws_anew():
+    """Each replay of a captured population step draws new masks."""
+    from blades_amd.engine import FusedEngine, ParamSpec
+    torch.manual_seed(0)
+    model = text_cct_2(seq_len=12, vocab_size=60, num_classes=60,
+                       word_embedding_dim=24, dropout=0.2, fused_norm=True,
+                       act_bits=8).cuda().train()
+    engine = FusedEngine(model, ParamSpec.from_module(model), "cuda",
+                         head_loss=True)
+    p = tuple(t.detach() for t in model.parameters())
+    x = torch.randint(1, 60, (3, 6, 12), device="cuda")
+    y = torch.randint(0, 60, (3, 6), device="cuda")
+    one = torch.ones(3, device="cuda")
+    step = engine._build_grad_fn(True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step(p, x, y, one * 1e6, one)
+    torch.cuda.current_stream().wait_stream(s)
+    hi = one * 1e6
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(p, x, y, hi, one)
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(t.isfinite().all() for t in out)
+        seen.append(out[-1].clone())
+        assert step(p, x, y, hi, one)[-1].isfinite().all()
+    assert not torch.equal(seen[0], seen[1])
+    assert not torch.equal(seen[1], seen[2])
